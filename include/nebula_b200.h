@@ -193,6 +193,37 @@ int neb_greedy_accept(const void* logits, int64_t row_stride, int32_t vocab, int
                       int32_t* argmax_out, int32_t* out_tokens, int32_t* out_count, int32_t* out_accepted,
                       void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------- log probabilities
+ * Log probability, rank and entropy of logits rows, and each row's most likely
+ * tokens, in one launch with no host synchronisation.  The reference reports
+ * no log probabilities: its post layer keeps torch.argmax of the same logits
+ * (swiftLLM/swiftllm/worker/layers/post_layer.py:72).  The Python face is
+ * nebulasd_b200.logprobs.token_logprobs.
+ *
+ * logits        [num_rows][row_stride] of `dtype` (NEB_DTYPE_*), the first
+ *               `vocab` of each row used; rows may start at any element
+ * token_ids     [num_rows] or NULL: the row's given token t, or -1 for none
+ * logprobs      [num_rows]: x_t - log(sum_j exp(x_j)); NaN without a token
+ * ranks         [num_rows]: 1 + the number of logits larger than x_t; 0
+ *               without a token (logprobs and ranks are NULL iff token_ids is)
+ * entropy       [num_rows]: -sum_j p_j log p_j in nats, or NULL
+ * num_top       0 .. min(vocab, NEB_MAX_TOP_LOGPROBS)
+ * top_ids, top_logprobs [num_rows][num_top]: the tokens of the largest
+ *               logits, largest first, ties by the lowest token id
+ * -inf logits (banned tokens) have probability 0.  A row that holds a NaN or
+ * +inf, or nothing but -inf, gets NaN for every floating result; its order is
+ * still defined (a NaN counts as the largest value, -0 equals +0).  A token
+ * outside [-1, vocab) is treated as -1 and recorded as bit 6 of *error_bits.
+ * Needs no workspace. */
+#define NEB_DTYPE_F16 0
+#define NEB_DTYPE_BF16 1
+#define NEB_DTYPE_F32 2
+#define NEB_MAX_TOP_LOGPROBS 32
+int neb_token_logprobs(const void* logits, int32_t dtype, int64_t row_stride, int32_t vocab,
+                       int32_t num_rows, const int32_t* token_ids, int32_t num_top, float* logprobs,
+                       int32_t* ranks, float* entropy, int32_t* top_ids, float* top_logprobs,
+                       uint32_t* error_bits, void* stream);
+
 /* ------------------------------------------------------------ prefill attention
  * Causal attention within each sequence of a packed prefill batch.  Replaces
  * flash_attn_varlen_func (swiftLLM/swiftllm/worker/layers/transformer_layer.py:7-32,

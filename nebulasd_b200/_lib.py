@@ -48,6 +48,8 @@ SIGNATURES = {
     "neb_greedy_accept_workspace_bytes": ([_i32], _sz),
     "neb_greedy_accept": ([_vp, _i64, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp,
                            _sz, _vp], ctypes.c_int),
+    "neb_token_logprobs": ([_vp, _i32, _i64, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+                           ctypes.c_int),
     "neb_prefill_attention_workspace_bytes": ([_i64, _i32, _i32, _i32], _sz),
     "neb_prefill_attention": ([_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i64, _i32, _i32, _i32, _i32, ctypes.c_float,
                                _vp, _i64, _vp, _sz, _vp], ctypes.c_int),

@@ -44,6 +44,7 @@ enum DeviceError : uint32_t {
   kErrTimeout = 1u << 3,      // a bounded wait gave up
   kErrInvalidRows = 1u << 4,  // greedy accept: a request's rows or output limit are invalid
   kErrBadSeqlens = 1u << 5,   // prefill: cu_seqlens not a valid split of the tokens (or past max_seqlen)
+  kErrTokenId = 1u << 6,      // token log probabilities: token outside [-1, vocab)
 };
 
 __host__ __device__ inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
