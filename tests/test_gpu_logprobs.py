@@ -134,6 +134,23 @@ def test_masks(dtype, cuda):
     assert abs(float(got.entropy[5]) - math.log(2)) < 1e-6
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 40, 500])
+def test_confident_rows_keep_their_precision(dtype, rows, cuda):
+    """log p = -log1p(r) of a nearly certain token, to the relative precision of r (``g`` as above)."""
+    from nebulasd_b200.logprobs import token_logprobs
+    vocab = 20000
+    logits, tokens = _logits(rows, rows, vocab, dtype, cuda, spread=1.0)
+    logits[torch.arange(rows), tokens.long()] = torch.linspace(12, 24, rows, device=cuda).to(dtype)
+    got = token_logprobs(logits, tokens, 1)
+    lp, rk, ent, ids, tops = oracle(logits, tokens.tolist(), 1)
+    g = (-(-vocab // 128) + 64) * 2.0 ** -24
+    for a, b in ((got.logprobs, lp), (got.entropy, ent), (got.top_logprobs, tops)):
+        a, b = a.double().cpu(), torch.as_tensor(b)
+        assert bool(((a - b).abs() <= 4 * g * b.abs()).all())
+    assert got.ranks.tolist() == [1] * rows and got.top_ids[:, 0].tolist() == tokens.tolist()
+
+
 def test_row_splits_give_one_answer(cuda):
     """A row's ids and rank do not depend on how many rows are scored with it, its sums only in rounding."""
     from nebulasd_b200.logprobs import token_logprobs
