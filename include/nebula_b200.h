@@ -300,6 +300,78 @@ int neb_rmsnorm_inplace(void* x, const void* weight, int64_t num_rows, int32_t h
 int neb_rotary_inplace(void* q, void* k, const void* cos, const void* sin, int32_t num_tokens,
                        int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, void* stream);
 
+/* ------------------------------------------------------------- block pool
+ * Copying, forking, freeing and compacting blocks of the paged cache, planned
+ * on the device from device-resident lists (no host synchronisation), for
+ * programs that branch: best-of-n, beams, several answers to one prompt.  The
+ * reference has no counterpart on its production path (its banks give every
+ * request blocks of its own).  Python face: nebulasd_b200.block_pool.
+ *
+ *   k/v cache    [num_blocks][tiles_per_block][block_size][token_bytes]: for the
+ *                layout above tiles_per_block = num_layers * num_kv_heads and
+ *                token_bytes = 256; token_bytes any multiple of 16
+ *   block_table  [block_table_rows][max_blocks_per_seq] int32, -1 where unused
+ *   seq_blocks   [block_table_rows] int32: entries of the row in use (0: empty row)
+ *   ref_counts   [num_blocks] int32: rows that use the block (0: free)
+ *
+ * The results do not depend on thread order: free blocks are taken lowest
+ * first, and counts are whole numbers.  What an operator refuses it leaves as
+ * it was and OR-s into *error_bits (device memory, optional): bit 0 block index
+ * out of range, bit 1 row out of range, bit 2 more blocks than
+ * max_blocks_per_seq, bit 4 invalid rows, lengths or token counts, bit 7 a block
+ * in use without a positive count, bit 8 too few free blocks, bit 9 copies in
+ * conflict.  Calls on one pool must be ordered; no list may be part of the pool's
+ * tables, and the tables may not overlap. */
+
+/* Block dst[i] gets the first num_tokens[i] tokens (null: all) of block src[i],
+ * all tiles, both planes; the rest of dst[i] keeps its contents.  A pair whose
+ * dst is another pair's dst, or whose src is another pair's dst, is left out
+ * (bit 9), one with a block or token count out of range too (bits 0, 4). */
+int neb_copy_blocks(void* k_cache, void* v_cache, int64_t num_blocks, int32_t tiles_per_block,
+                    int32_t block_size, int32_t token_bytes, const int32_t* src, const int32_t* dst,
+                    const int32_t* num_tokens, int32_t num_pairs, uint32_t* error_bits, void* stream);
+
+/* Child i becomes a sequence of its own that starts with the first seq_lens[i]
+ * tokens of row parents[i]: its row children[i] (empty before) shares the
+ * parent's full blocks below seq_lens[i] (their counts rise by one), and gets
+ * fresh blocks for the rest of max(seq_lens[i], capacities[i]) tokens
+ * (capacities null: of seq_lens[i]); the first of them gets a copy of the
+ * tokens of the partial block.  So neither side ever appends to a block that the
+ * other can see.  With seq_lens[i] = 0 it is an allocation, and parents[i] is
+ * not read.  Fresh blocks go to the children in their order, lowest first; a
+ * child whose turn comes after the free blocks are spent is refused (bit 8).
+ * Refused as well: a row that is not empty, or listed again after its first
+ * time, a length beyond the parent's blocks (bit 4).  A refused child's row
+ * stays empty.  An entry of the parent out of range is copied as -1 (bit 0).
+ * Workspace: neb_fork_workspace_bytes, 16-byte aligned, any contents. */
+size_t neb_fork_workspace_bytes(int64_t num_blocks, int32_t num_children);
+int neb_fork_sequences(void* k_cache, void* v_cache, int64_t num_blocks, int32_t tiles_per_block,
+                       int32_t block_size, int32_t token_bytes, int32_t* block_table,
+                       int32_t block_table_rows, int32_t max_blocks_per_seq, int32_t* seq_blocks,
+                       int32_t* ref_counts, const int32_t* parents, const int32_t* children,
+                       const int32_t* seq_lens, const int32_t* capacities, int32_t num_children,
+                       void* workspace, size_t workspace_bytes, uint32_t* error_bits, void* stream);
+
+/* Empties the listed rows: the counts of their blocks fall by one (a block
+ * whose count reaches 0 is free), their entries in use become -1, their
+ * seq_blocks 0.  A row listed twice is freed once; an empty row stays empty. */
+int neb_free_sequences(int32_t* block_table, int32_t block_table_rows, int32_t max_blocks_per_seq,
+                       int32_t* seq_blocks, int32_t* ref_counts, int64_t num_blocks, const int32_t* rows,
+                       int32_t num_rows, uint32_t* error_bits, void* stream);
+
+/* Moves the blocks in use to the front: with n of them, the i-th block in use
+ * at or above index n goes to the i-th free block below n, with its contents
+ * and count, and every row's entries follow.  Afterwards blocks n.. are free,
+ * one contiguous range (as HostKV copies want them).  new_index [num_blocks]
+ * gets each block's new index, -1 for a block that was free.
+ * Workspace: neb_compact_workspace_bytes, 16-byte aligned, any contents. */
+size_t neb_compact_workspace_bytes(int64_t num_blocks);
+int neb_compact_blocks(void* k_cache, void* v_cache, int64_t num_blocks, int32_t tiles_per_block,
+                       int32_t block_size, int32_t token_bytes, int32_t* block_table,
+                       int32_t block_table_rows, int32_t max_blocks_per_seq, int32_t* seq_blocks,
+                       int32_t* ref_counts, int32_t* new_index, void* workspace, size_t workspace_bytes,
+                       uint32_t* error_bits, void* stream);
+
 /* ------------------------------------------------------------ HostKV copies
  * direction 0 = D2H (writeback), 1 = H2D (restore).  regions: host array of
  * num_regions triples (host_block, gpu_block, block_count), host_block

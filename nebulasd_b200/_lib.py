@@ -50,6 +50,14 @@ SIGNATURES = {
                            _sz, _vp], ctypes.c_int),
     "neb_token_logprobs": ([_vp, _i32, _i64, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
                            ctypes.c_int),
+    "neb_copy_blocks": ([_vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _i32, _vp, _vp], ctypes.c_int),
+    "neb_fork_workspace_bytes": ([_i64, _i32], _sz),
+    "neb_fork_sequences": ([_vp, _vp, _i64, _i32, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i32,
+                            _vp, _sz, _vp, _vp], ctypes.c_int),
+    "neb_free_sequences": ([_vp, _i32, _i32, _vp, _vp, _i64, _vp, _i32, _vp, _vp], ctypes.c_int),
+    "neb_compact_workspace_bytes": ([_i64], _sz),
+    "neb_compact_blocks": ([_vp, _vp, _i64, _i32, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _sz, _vp, _vp],
+                           ctypes.c_int),
     "neb_prefill_attention_workspace_bytes": ([_i64, _i32, _i32, _i32], _sz),
     "neb_prefill_attention": ([_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i64, _i32, _i32, _i32, _i32, ctypes.c_float,
                                _vp, _i64, _vp, _sz, _vp], ctypes.c_int),

@@ -78,3 +78,44 @@ def error_word(device: torch.device) -> torch.Tensor:
                 t = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
             _error_words[index] = t
         return t
+
+
+class ErrorWords:
+    """One int32 word per device where an operator's kernels record error bits (never a trap), for
+    operators that keep no workspace of their own."""
+
+    def __init__(self, what: str) -> None:
+        self._what, self._words = what, {}
+
+    def word(self, index: int) -> torch.Tensor:
+        t = self._words.get(index)
+        if t is not None:
+            return t
+        with _lock:
+            t = self._words.get(index)
+            if t is None:
+                t = self._words[index] = new_error_word(index, self._what)
+        return t
+
+    def read(self, device: torch.device | None = None) -> int:
+        """Synchronise the device's current stream; return and clear the bits recorded so far."""
+        index = device.index if device is not None and device.index is not None else torch.cuda.current_device()
+        return read_error_word(self.word(index))
+
+
+def new_error_word(index: int, what: str) -> torch.Tensor:
+    with torch.cuda.device(index):
+        # Inside a capture its zero fill would run at each replay and not now.
+        if torch.cuda.is_current_stream_capturing():
+            raise _lib.NebError(f"{what}: its first call on a device must come before any graph capture")
+        with torch.inference_mode(False):  # see attention_workspace
+            t = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
+        torch.cuda.current_stream(index).synchronize()  # every stream uses the word from here on
+    return t
+
+
+def read_error_word(t: torch.Tensor) -> int:
+    bits = int(t.item()) & 0xFFFFFFFF
+    if bits:
+        t.zero_()
+    return bits

@@ -45,6 +45,9 @@ enum DeviceError : uint32_t {
   kErrInvalidRows = 1u << 4,  // greedy accept: a request's rows or output limit are invalid
   kErrBadSeqlens = 1u << 5,   // prefill: cu_seqlens not a valid split of the tokens (or past max_seqlen)
   kErrTokenId = 1u << 6,      // token log probabilities: token outside [-1, vocab)
+  kErrRefCount = 1u << 7,     // block pool: a block in use whose reference count is not positive
+  kErrNoFreeBlock = 1u << 8,  // block pool: a fork found too few free blocks
+  kErrCopyConflict = 1u << 9,  // block copies: a block is another pair's destination too
 };
 
 __host__ __device__ inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }

@@ -10,19 +10,18 @@ in one launch and without a host sync.  (The reference keeps only
 """
 from __future__ import annotations
 
-import threading
 from typing import NamedTuple
 
 import torch
 
 from . import _lib
+from ._workspace import ErrorWords
 from .kernels.paged_attn import _raw_stream
 
 MAX_TOP = 32  # NEB_MAX_TOP_LOGPROBS
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
-_lock = threading.Lock()
-_words: dict[int, torch.Tensor] = {}
+_errors = ErrorWords("token_logprobs")
 
 
 class TokenLogprobs(NamedTuple):
@@ -31,22 +30,6 @@ class TokenLogprobs(NamedTuple):
     entropy: torch.Tensor              # [R] fp32, nats
     top_ids: torch.Tensor | None       # [R, num_top] int32, None when num_top is 0
     top_logprobs: torch.Tensor | None  # [R, num_top] fp32
-
-
-def _error_word(index: int) -> torch.Tensor:
-    t = _words.get(index)
-    if t is None:
-        with _lock:
-            t = _words.get(index)
-            if t is None:
-                if torch.cuda.is_current_stream_capturing():
-                    raise _lib.NebError("call token_logprobs once on this device before capturing it into a graph")
-                with torch.inference_mode(False):
-                    t = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
-                # Every stream uses the word from here on.
-                torch.cuda.current_stream(index).synchronize()
-                _words[index] = t
-    return t
 
 
 def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor | None = None, num_top: int = 0) -> TokenLogprobs:
@@ -96,7 +79,7 @@ def _launch(logits, token_ids, num_top, rows, vocab, index) -> TokenLogprobs:
     rc = _lib.lib.neb_token_logprobs(
         logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), vocab, rows, _lib.ptr(token_ids), num_top,
         _lib.ptr(logprobs), _lib.ptr(ranks), entropy.data_ptr(), _lib.ptr(top_ids), _lib.ptr(top_logprobs),
-        _error_word(index).data_ptr(), _raw_stream(index))
+        _errors.word(index).data_ptr(), _raw_stream(index))
     _lib.check(rc, "token_logprobs")
     return TokenLogprobs(logprobs, ranks, entropy, top_ids, top_logprobs)
 
@@ -104,9 +87,4 @@ def _launch(logits, token_ids, num_top, rows, vocab, index) -> TokenLogprobs:
 def workspace_errors(device: torch.device | None = None) -> int:
     """Synchronise the device's current stream and return (and clear) the error bits that
     calls on it recorded (bit 6: a token outside ``[-1, vocab)``)."""
-    index = device.index if device is not None and device.index is not None else torch.cuda.current_device()
-    word = _error_word(index)
-    bits = int(word.item()) & 0xFFFFFFFF
-    if bits:
-        word.zero_()
-    return bits
+    return _errors.read(device)

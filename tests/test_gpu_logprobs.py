@@ -148,7 +148,7 @@ def test_confident_rows_keep_their_precision(dtype, rows, cuda):
     for a, b in ((got.logprobs, lp), (got.entropy, ent), (got.top_logprobs, tops)):
         a, b = a.double().cpu(), torch.as_tensor(b)
         assert bool(((a - b).abs() <= 4 * g * b.abs()).all())
-    assert got.ranks.tolist() == [1] * rows and got.top_ids[:, 0].tolist() == tokens.tolist()
+    assert got.ranks.tolist() == rk.tolist() and got.top_ids.tolist() == ids.tolist()
 
 
 def test_row_splits_give_one_answer(cuda):
