@@ -11,17 +11,17 @@
 // confident row has log p = -log1p(r) with r << 1, which 1 + r would round away.
 //
 // A row is streamed by a cluster of S CTAs (S = 1 when the rows alone fill the
-// GPU), each through a ring of 16 KB tiles filled by bulk asynchronous copies
+// GPU), each through a ring of 32 KB tiles filled by bulk asynchronous copies
 // while the tiles before are summed from registers: the row is read once, the
 // ring keeps the loads in flight whatever the arithmetic does.  The CTAs leave
 // their sums and candidates in the first CTA's shared memory, so there is no
 // workspace and no second launch.
 //
-// Alternatives: a CTA keeps a list of candidates and a threshold that at least
-// num_top logits reach.  A tile's threads compare their own tile maximum (needed
-// for m anyway) with the threshold, and only a thread above it looks at its
-// logits again, so after the first tile almost no tile costs more than the
-// barrier it needs to free its ring slot.
+// Alternatives: a CTA keeps a list of candidates and a threshold, the num_top-th
+// of them.  A thread compares its tile maximum (needed for m anyway) with the
+// threshold, and only where it is higher does the warp look at that thread's
+// logits again, in the ring.  So after the first tile a tile costs its barrier and
+// a few candidates.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -33,14 +33,14 @@ namespace logprobs {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kWords = 4;                          // 16-byte words per thread and tile
-constexpr int kTileWords = kThreads * kWords;      // 16 KB
-constexpr int kStages = 3;
+constexpr int kWords = 8;                          // 16-byte words per thread and tile
+constexpr int kTileWords = kThreads * kWords;      // 32 KB
+constexpr int kStages = 2;
 constexpr int kMaxTop = NEB_MAX_TOP_LOGPROBS;
 constexpr int kMaxSplits = 8;                      // CTAs per row (the portable cluster size)
-constexpr int kKeep = 64;                          // candidates left by a prune (at most)
-constexpr int kList = kKeep + kMaxTop * kWords * 8;  // plus every logit of kMaxTop threads' tile
-constexpr int kPruneAt = 192;                      // candidates from which a prune pays
+constexpr int kPruneAt = 16;                       // candidates beyond num_top from which a prune pays
+constexpr int kRound = 2;                          // words of a thread that an overfull tile lists at a time
+constexpr int kList = kMaxTop + kPruneAt + kMaxTop * kRound * 8;  // and those of kMaxTop threads
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr long long kWaitLimit = 4000000000ll;     // cycles (about 2 s)
@@ -63,8 +63,9 @@ struct Params {
 // One CTA's part of a row: its maximum, the sums about it (r without the maximum itself).
 struct Part {
   float m, r, w;
-  int above;
+  int above;  // logits larger than the given token's (bit 31: see kSkipped)
 };
+constexpr int kSkipped = INT_MIN;  // a tile below kLow was left out
 
 struct Shared {
   uint4 ring[kStages][kTileWords];
@@ -76,10 +77,17 @@ struct Shared {
   u64 warp_key[kWarps];
   float warp_f[3][kWarps];
   int warp_count[2][kWarps], warp_above[kWarps];
-  int n, owner;
+  int n;
 };
 
 // ------------------------------------------------------------------- elements
+// Keeps a NaN, unlike fmaxf.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 template <typename T>
 struct Elem;
 
@@ -99,91 +107,73 @@ __device__ __forceinline__ u64 make_key(float x, int idx) {
 __device__ __forceinline__ int key_index(u64 key) { return (int)~(unsigned int)key; }
 __device__ __forceinline__ float key_value(u64 key) { return value_of_order((unsigned int)(key >> 32)); }
 
+// The one-pass sums are for rows whose maximum lies in [kLowRow, kHighRow], where the rounding of m log2 e
+// stays small and clamped differences finite; other rows go to general_row.  Logits below kLow (masks by a
+// large negative number) are never a reference: beside such a maximum their share is exp(-1000) or less.
+constexpr float kLow = -65000.f, kLowRow = -64000.f, kHighRow = 66000.f;
+constexpr float kFinite = -65504.f;
+
 template <>
 struct Elem<__half> {
+  typedef __half2 Two;
   static constexpr int kPerWord = 8;
   static constexpr unsigned int kLowest = 0xfc00fc00u;  // -inf pair
+  static constexpr float kUlp = 1.f / 512.f;  // of the type, relative
   static __device__ __forceinline__ float load(const void* p, long long i) {
     return __half2float(static_cast<const __half*>(p)[i]);
   }
   static __device__ __forceinline__ float2 pair(unsigned int u) { return h2_to_f2(u); }
-  static __device__ __forceinline__ float get(const uint4& v, int j) {
-    const unsigned int u = j < 4 ? (j < 2 ? v.x : v.y) : (j < 6 ? v.z : v.w);
-    return __half2float(__ushort_as_half((unsigned short)((j & 1) ? u >> 16 : u)));
-  }
+  static __device__ __forceinline__ Two twice(float x) { return __float2half2_rn(x); }
 };
 template <>
 struct Elem<__nv_bfloat16> {
+  typedef __nv_bfloat162 Two;
   static constexpr int kPerWord = 8;
   static constexpr unsigned int kLowest = 0xff80ff80u;
+  static constexpr float kUlp = 1.f / 64.f;  // of the type, relative
   static __device__ __forceinline__ float load(const void* p, long long i) {
     return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
   }
   static __device__ __forceinline__ float2 pair(unsigned int u) {
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
   }
-  static __device__ __forceinline__ float get(const uint4& v, int j) {
-    const unsigned int u = j < 4 ? (j < 2 ? v.x : v.y) : (j < 6 ? v.z : v.w);
-    return __uint_as_float((j & 1) ? u & 0xffff0000u : u << 16);
-  }
+  static __device__ __forceinline__ Two twice(float x) { return __float2bfloat162_rn(x); }
 };
 template <>
 struct Elem<float> {
   static constexpr int kPerWord = 4;
   static constexpr unsigned int kLowest = 0xff800000u;
+  static constexpr float kUlp = 0.f;  // of the type, relative
   static __device__ __forceinline__ float load(const void* p, long long i) { return static_cast<const float*>(p)[i]; }
-  static __device__ __forceinline__ float get(const uint4& v, int j) {
-    return __uint_as_float(j < 2 ? (j == 0 ? v.x : v.y) : (j == 2 ? v.z : v.w));
-  }
 };
 
-// The two elements (of a pair word for 16-bit types, of two words for fp32) at position j of a word.
-template <typename T>
-__device__ __forceinline__ float2 word_pair(const uint4& v, int j) {
-  if constexpr (Elem<T>::kPerWord == 8) {
-    return Elem<T>::pair(j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w);
-  } else {
-    return j == 0 ? make_float2(__uint_as_float(v.x), __uint_as_float(v.y))
-                  : make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
-  }
+// The 32-bit piece q of a word, and its one or two logits.
+__device__ __forceinline__ unsigned int piece(const uint4& v, int q) {
+  return q == 0 ? v.x : q == 1 ? v.y : q == 2 ? v.z : v.w;
 }
+// NaN if there is one.
 template <typename T>
 __device__ __forceinline__ float words_max(const uint4 (&v)[kWords]) {
   if constexpr (Elem<T>::kPerWord == 4) {
-    float m = __int_as_float(0xff800000);
+    float m = neg_inf();
 #pragma unroll
-    for (int u = 0; u < kWords; ++u) {
-      m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(v[u].x), __uint_as_float(v[u].y)),
-                         fmaxf(__uint_as_float(v[u].z), __uint_as_float(v[u].w))));
-    }
+    for (int u = 0; u < kWords; ++u)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) m = max_nan(m, __uint_as_float(piece(v[u], q)));
     return m;
-  } else if constexpr (sizeof(T) == 2 && Elem<T>::kLowest == 0xfc00fc00u) {
-    __half2 m = __halves2half2(__ushort_as_half(0xfc00u), __ushort_as_half(0xfc00u));
-#pragma unroll
-    for (int u = 0; u < kWords; ++u) {
-      const unsigned int q[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) m = __hmax2(m, *reinterpret_cast<const __half2*>(&q[i]));
-    }
-    return fmaxf(__low2float(m), __high2float(m));
   } else {
-    const unsigned int low = 0xff80ff80u;
-    __nv_bfloat162 m = *reinterpret_cast<const __nv_bfloat162*>(&low);
+    typedef typename Elem<T>::Two Two;
+    const unsigned int low = Elem<T>::kLowest;
+    Two m = *reinterpret_cast<const Two*>(&low);
 #pragma unroll
-    for (int u = 0; u < kWords; ++u) {
-      const unsigned int q[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+    for (int u = 0; u < kWords; ++u)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) m = __hmax2(m, *reinterpret_cast<const __nv_bfloat162*>(&q[i]));
-    }
-    return fmaxf(__low2float(m), __high2float(m));
+      for (int q = 0; q < 4; ++q) {
+        const unsigned int x = piece(v[u], q);
+        m = __hmax2_nan(m, *reinterpret_cast<const Two*>(&x));
+      }
+    return max_nan(__low2float(m), __high2float(m));
   }
-}
-
-// Keeps a NaN, unlike fmaxf: a NaN logit has to reach the sums.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
 }
 
 // Two fp32 lanes per instruction (sm_100).
@@ -213,8 +203,79 @@ __device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
   return r;
 }
 
-// (from - to) log2 e for moving a reference up, finite also from an empty part (-inf).
-__device__ __forceinline__ float step_down(float from, float to) { return fmaxf((from - to) * kLog2e, -1000.f); }
+// A step of the exponent's reference, finite also from an empty part (-inf).
+__device__ __forceinline__ float bounded(float step) { return fmaxf(step, -1000.f); }
+
+__device__ __forceinline__ float warp_max_nan(float v) {
+  float r;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// The exponents' reference: t = x log2 e - mc with mc the rounded m log2 e, one fma per logit.  t of m
+// itself is t0, not 0; e0 = 2^t0 takes that out of the finished sums.
+__device__ __forceinline__ float exponent(float x, float mc) { return fmaf(x, kLog2e, -mc); }
+
+// Adds a tile's terms 2^t and 2^t t, two fp32 lanes per instruction.  Logits far below the reference count
+// as 100 below it: 2^t is 0 all the same, and 0 times -inf is kept out of the second one.
+template <typename T>
+__device__ __forceinline__ void add_tile(const uint4 (&v)[kWords], float m, float mc, u64 (&s)[2], u64 (&w)[2]) {
+  const u64 c2 = pack2(kLog2e, kLog2e), mc2 = pack2(-mc, -mc);
+  const float lo = fmaxf(m - 100.f - fabsf(m) * Elem<T>::kUlp, kFinite);
+  auto add = [&](float a, float b, int i) {
+    const u64 t = fma2(pack2(a, b), c2, mc2);
+    const float2 f = unpack2(t);
+    const u64 e = pack2(fast_exp2(f.x), fast_exp2(f.y));
+    s[i] = add2(s[i], e);
+    w[i] = fma2(e, t, w[i]);
+  };
+  if constexpr (Elem<T>::kPerWord == 4) {
+#pragma unroll
+    for (int u = 0; u < kWords; ++u) {
+      add(fmaxf(__uint_as_float(v[u].x), lo), fmaxf(__uint_as_float(v[u].y), lo), 0);
+      add(fmaxf(__uint_as_float(v[u].z), lo), fmaxf(__uint_as_float(v[u].w), lo), 1);
+    }
+  } else {
+    typedef typename Elem<T>::Two Two;
+    const Two lo2 = Elem<T>::twice(lo);
+#pragma unroll
+    for (int u = 0; u < kWords; ++u)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const unsigned int x = piece(v[u], q);
+        const Two h = __hmax2(*reinterpret_cast<const Two*>(&x), lo2);
+        const float2 f = Elem<T>::pair(*reinterpret_cast<const unsigned int*>(&h));
+        add(f.x, f.y, q & 1);
+      }
+  }
+}
+
+// Logits of a tile larger than `given`.
+template <typename T>
+__device__ __forceinline__ int count_above(const uint4 (&v)[kWords], float given) {
+  if constexpr (Elem<T>::kPerWord == 4) {
+    int n = 0;
+#pragma unroll
+    for (int u = 0; u < kWords; ++u)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) n += __uint_as_float(piece(v[u], q)) > given;
+    return n;
+  } else {
+    typedef typename Elem<T>::Two Two;
+    const Two g = Elem<T>::twice(given);  // exact: it is one of the logits
+    // Masks 0xffff add up to 65536 (low - high) - low in 32 bits.
+    unsigned int sum = 0;
+#pragma unroll
+    for (int u = 0; u < kWords; ++u)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const unsigned int x = piece(v[u], q);
+        sum += __hgt2_mask(*reinterpret_cast<const Two*>(&x), g);
+      }
+    const int low = (int)(-sum & 0xffffu);
+    return 2 * low - ((int)(sum + low) >> 16);
+  }
+}
 
 // Untiled bulk copy into shared memory, completing on `bar`.
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -269,18 +330,29 @@ __device__ __forceinline__ u64 search(Shared& sh, int& turn, u64 lo, int lowest,
   return lo;
 }
 
-// Leaves between num_top and kKeep of the list's n > kKeep candidates; returns the new threshold.
-__device__ __noinline__ u64 prune(Shared& sh, int n, int num_top, int& turn) {
+// The list's num_top largest keys in order (0 where there are fewer) into sh.sorted, by counting: n <= kThreads.
+__device__ __forceinline__ void rank_list(Shared& sh, int n, int num_top) {
+  const int tid = threadIdx.x;
+  if (n < num_top && tid >= n && tid < num_top) sh.sorted[tid] = 0;
+  if (tid < n) {
+    const u64 key = sh.list[tid];
+    int before = 0;
+    for (int j = 0; j < n; ++j) before += sh.list[j] > key;
+    if (before < num_top) sh.sorted[before] = key;
+  }
+  __syncthreads();
+}
+
+// Shortens a list of n > kThreads candidates to at most kThreads, num_top or more.
+__device__ __noinline__ int shorten(Shared& sh, int n, int num_top, int& turn) {
   constexpr int kEach = (kList + kThreads - 1) / kThreads;
   u64 key[kEach];
-  int mine = 0;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int at = threadIdx.x + i * kThreads;
     key[i] = at < n ? sh.list[at] : 0;
   }
-  mine = kEach;
-  const u64 thr = search(sh, turn, 0, num_top, kKeep, mine, [&](int i) { return key[i]; });
+  const u64 thr = search(sh, turn, 0, num_top, kThreads, kEach, [&](int i) { return key[i]; });
   __syncthreads();
   if (threadIdx.x == 0) sh.n = 0;
   __syncthreads();
@@ -288,24 +360,20 @@ __device__ __noinline__ u64 prune(Shared& sh, int n, int num_top, int& turn) {
   for (int i = 0; i < kEach; ++i)
     if (key[i] > thr) sh.list[atomicAdd(&sh.n, 1)] = key[i];
   __syncthreads();
-  return thr;
+  n = sh.n;
+  return n;
 }
 
-// The list's num_top largest keys, in order, into sh.sorted (0 where there are fewer).
-__device__ __forceinline__ void sort_top(Shared& sh, int n, int num_top, int& turn) {
-  if (n > kKeep) {
-    prune(sh, n, num_top, turn);
-    n = sh.n;
-  }
-  if (threadIdx.x < num_top) sh.sorted[threadIdx.x] = 0;
+// Leaves the num_top largest of the list's n >= num_top candidates, in order; returns the last of them,
+// which is the threshold from here on.
+__device__ __forceinline__ u64 prune(Shared& sh, int n, int num_top, int& turn) {
+  if (n > kThreads) n = shorten(sh, n, num_top, turn);
+  rank_list(sh, n, num_top);
+  if (threadIdx.x < num_top) sh.list[threadIdx.x] = sh.sorted[threadIdx.x];
+  if (threadIdx.x == 0) sh.n = num_top;
+  const u64 last = sh.sorted[num_top - 1];
   __syncthreads();
-  if ((int)threadIdx.x < n) {
-    const u64 key = sh.list[threadIdx.x];
-    int before = 0;
-    for (int j = 0; j < n; ++j) before += sh.list[j] > key;
-    if (before < num_top) sh.sorted[before] = key;
-  }
-  __syncthreads();
+  return last;
 }
 
 // Joins `b` into `a`: sums about the larger maximum, which alone is left out of r.
@@ -315,30 +383,57 @@ __device__ __forceinline__ Part join(Part a, Part b) {
     a = b;
     b = t;
   }
-  const float dt = step_down(b.m, a.m), f = fast_exp2(dt);
+  const float dt = bounded((b.m - a.m) * kLog2e), f = fast_exp2(dt);
   const float s = b.m == neg_inf() ? b.r : 1.f + b.r;  // b's maximum is an ordinary term now
   a.r += f * s;
   a.w += f * (b.w + s * dt);
-  a.above += b.above;
+  a.above = ((a.above + b.above) & INT_MAX) | ((a.above | b.above) & kSkipped);
   return a;
 }
 
-// A row with a NaN or +inf, by the first CTA alone: results NaN, order over all values (NaN highest).
+// Any row, logit by logit, by one CTA: rows with a NaN or +inf (results NaN, order over all values) and rows
+// that have nothing above kLow.
 template <typename T>
-__device__ __noinline__ void unordered_row(Shared& sh, const Params& p, const void* x, int row, int tok) {
+__device__ __noinline__ void general_row(Shared& sh, const Params& p, const void* x, int row, int tok) {
   const int tid = threadIdx.x;
   const float nan = __int_as_float(0x7fffffff);
-  int turn = 0;
-  int above = 0;
-  if (tok >= 0) {
-    const unsigned int given = order_f32(Elem<T>::load(x, tok));
-    for (int j = tid; j < p.vocab; j += kThreads) above += order_f32(Elem<T>::load(x, j)) > given;
+  int turn = 0, above = 0;
+  float m = neg_inf();
+  const unsigned int given = tok >= 0 ? order_f32(Elem<T>::load(x, tok)) : ~0u;
+  for (int j = tid; j < p.vocab; j += kThreads) {
+    const float v = Elem<T>::load(x, j);
+    above += order_f32(v) > given;
+    m = fmaxf(m, v);
   }
   above = block_count(sh, above, turn);
+  m = warp_max_nan(m);
+  if ((tid & 31) == 0) sh.warp_f[0][tid >> 5] = m;
+  __syncthreads();
+  for (int i = 0; i < kWarps; ++i) m = fmaxf(m, sh.warp_f[0][i]);
+  float s = 0.f, w = 0.f;
+  for (int j = tid; j < p.vocab; j += kThreads) {
+    const float t = (Elem<T>::load(x, j) - m) * kLog2e;  // NaN where the row's results are
+    const float e = fast_exp2(t);
+    s += e;
+    if (!(e == 0.f)) w = fmaf(e, t, w);
+  }
+  s = warp_sum(s);
+  w = warp_sum(w);
+  if ((tid & 31) == 0) {
+    sh.warp_f[1][tid >> 5] = s;
+    sh.warp_f[2][tid >> 5] = w;
+  }
+  __syncthreads();
+  s = w = 0.f;
+  for (int i = 0; i < kWarps; ++i) {
+    s += sh.warp_f[1][i];
+    w += sh.warp_f[2][i];
+  }
+  const float ln_s = s > 0.f ? logf(s) : nan;
   if (tid == 0) {
-    if (p.logprobs) p.logprobs[row] = nan;
+    if (p.logprobs) p.logprobs[row] = tok >= 0 ? (Elem<T>::load(x, tok) - m) - ln_s : nan;
     if (p.ranks) p.ranks[row] = tok >= 0 ? 1 + above : 0;
-    if (p.entropy) p.entropy[row] = nan;
+    if (p.entropy) p.entropy[row] = ln_s - kLn2 * (w / s);
   }
   u64 limit = ~0ull;
   for (int k = 0; k < p.num_top; ++k) {
@@ -359,7 +454,7 @@ __device__ __noinline__ void unordered_row(Shared& sh, const Params& p, const vo
     for (int i = 0; i < kWarps; ++i) limit = sh.warp_key[i] > limit ? sh.warp_key[i] : limit;
     if (tid == 0) {
       p.top_ids[(long long)row * p.num_top + k] = key_index(limit);
-      p.top_logprobs[(long long)row * p.num_top + k] = nan;
+      p.top_logprobs[(long long)row * p.num_top + k] = (key_value(limit) - m) - ln_s;
     }
   }
 }
@@ -370,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Param
   extern __shared__ __align__(128) unsigned char smem_raw[];
   Shared& sh = *reinterpret_cast<Shared*>(smem_raw);
   constexpr int kPer = Elem<T>::kPerWord;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int splits = p.splits, row = blockIdx.x / splits, part = blockIdx.x - row * splits;
   const T* x = static_cast<const T*>(p.logits) + (long long)row * p.row_stride;
   const int k = p.num_top;
@@ -406,21 +501,54 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Param
   const float given = tok >= 0 ? Elem<T>::load(x, tok) : __int_as_float(0x7f800000);
   __syncthreads();
 
-  float m = neg_inf(), s = 0.f, w = 0.f;  // sums about m, without the tile that holds m:
-  float p_ref = 0.f;                      // that tile's sum
-  int ref_tile = -1;                      // (-1: a head or tail logit, alone)
+  // Per warp: the reference m, rounded to mc in base 2.  Per lane: sums of the tiles since the one that
+  // holds m (acc_*), of the tiles before it (s, w) and of that tile itself (p_ref), which is kept
+  // apart because it is summed again without m in the end.
+  float m = neg_inf(), mc = 0.f, s = 0.f, w = 0.f, p_ref = 0.f;
+  u64 acc_s[2] = {0, 0}, acc_w[2] = {0, 0};
+  int ref_tile = -1;  // (-1: the head and tail logits)
   int above = 0;
-  u64 thr = 0;                            // at least k logits of this CTA are above it (0: not known yet)
-  int n = k && part == 0 ? head + tail : 0;  // candidates listed so far
+  bool skipped = false;
+  u64 thr = 0;        // the k-th largest candidate (0: not known yet)
+  int n = k && part == 0 ? head + tail : 0;  // candidates listed
   int turn = 0;
-  if (part == 0 && tid < head + tail) {
-    const int j = tid < head ? tid : head + words * kPer + (tid - head);
-    const float v = Elem<T>::load(x, j);
-    if (v > m) m = v;
-    const float t = max_nan((v - (m == neg_inf() ? 0.f : m)) * kLog2e, -200.f);
-    p_ref = fast_exp2(t);
-    above = v > given;
-    if (k) sh.list[atomicAdd(&sh.n, 1)] = make_key(v, j);
+  auto flush = [&]() {
+    const float2 a = unpack2(add2(acc_s[0], acc_s[1])), b = unpack2(add2(acc_w[0], acc_w[1]));
+    s += a.x + a.y;
+    w += b.x + b.y;
+    acc_s[0] = acc_s[1] = acc_w[0] = acc_w[1] = 0;
+  };
+  auto raise_to = [&](float top, int tile) {  // s, w and p_ref move to the reference `top`
+    const float to = top * kLog2e, dt = bounded(m == neg_inf() ? -1000.f : mc - to), f = fast_exp2(dt);
+    const float all = s + p_ref;
+    w = f * fmaf(all, dt, w);
+    s = f * all;
+    p_ref = 0.f;
+    m = top;
+    mc = to;
+    ref_tile = tile;
+  };
+  float lone = neg_inf();  // a lane's head or tail logit
+  if (part == 0 && warp == 0) {
+    if (lane < head + tail) {
+      const int j = lane < head ? lane : head + words * kPer + (lane - head);
+      lone = Elem<T>::load(x, j);
+      above = lone > given;
+      if (k) sh.list[atomicAdd(&sh.n, 1)] = make_key(lone, j);
+    }
+    __syncwarp();
+    const float top = warp_max_nan(lone != lone ? neg_inf() : lone);
+    if (top >= kLow) {
+      raise_to(top, -1);
+      if (!(lone < kLow)) {
+        const float t = exponent(fmaxf(lone, m - 100.f), mc), e = lone != lone ? lone : fast_exp2(t);
+        p_ref = e;
+        w = e * t;
+      }
+    } else if (top > neg_inf()) {
+      skipped = true;
+    }
+    if (lone != lone) s = lone;
   }
 
   bool late = false;
@@ -435,78 +563,61 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Param
       v[u] = a < nw ? sh.ring[st][a]
                     : make_uint4(Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest);
     }
-    const float tm = words_max<T>(v);
-    const float mn = fmaxf(m, tm);
-    {
-      const float mm = mn == neg_inf() ? 0.f : mn;
-      const u64 neg_m = pack2(-mm, -mm), c2 = pack2(kLog2e, kLog2e);
-      u64 s0 = 0, s1 = 0, q0 = 0, q1 = 0;
-#pragma unroll
-      for (int u = 0; u < kWords; ++u) {
-#pragma unroll
-        for (int j = 0; j < kPer / 2; ++j) {
-          const float2 f = word_pair<T>(v[u], j);
-          const float2 t = unpack2(mul2(add2(pack2(f.x, f.y), neg_m), c2));
-          const float tx = max_nan(t.x, -200.f), ty = max_nan(t.y, -200.f);
-          const u64 e = pack2(fast_exp2(tx), fast_exp2(ty));
-          if (j & 1) {
-            s1 = add2(s1, e);
-            q1 = fma2(e, pack2(tx, ty), q1);
-          } else {
-            s0 = add2(s0, e);
-            q0 = fma2(e, pack2(tx, ty), q0);
-          }
-        }
-      }
-      const float2 sp = unpack2(add2(s0, s1)), qp = unpack2(add2(q0, q1));
-      const float ps = sp.x + sp.y, pw = qp.x + qp.y;
-      if (tm > m) {
-        const float dt = step_down(m, mn), f = fast_exp2(dt), all = s + p_ref;
-        w = fmaf(f, fmaf(all, dt, w), pw);
-        s = f * all;
-        p_ref = ps;
-        ref_tile = i;
-        m = mn;
-      } else {
-        s += ps;
-        w += pw;
-      }
+    const float tm = words_max<T>(v), top = warp_max_nan(tm);
+    const bool raise = top > m && top >= kLow;
+    if (raise) {
+      flush();
+      raise_to(top, i);
     }
-    if (__any_sync(~0u, tm > given)) {
-#pragma unroll
-      for (int u = 0; u < kWords; ++u)
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) above += Elem<T>::get(v[u], j) > given;
+    // A tile far below the reference (banned tokens) adds nothing.
+    if (top >= m - 120.f) add_tile<T>(v, m, mc, acc_s, acc_w);
+    if (top != top) s = top;
+    else if (m == neg_inf() && top > neg_inf()) skipped = true;
+    if (raise) {
+      const float2 a = unpack2(add2(acc_s[0], acc_s[1]));
+      p_ref = a.x + a.y;
+      acc_s[0] = acc_s[1] = 0;
     }
+    if (top > given) above += count_above<T>(v, given);
     if (k == 0) {
-      __syncthreads();
+      __syncthreads();  // the ring slot is read
       if (tid == 0 && i + kStages < tiles) fill(i + kStages);
       continue;
     }
     // ---- candidates
     const int base = head + (w0 + i * kTileWords + tid) * kPer;  // index of the thread's first logit
     const bool some = tid < nw;
-    bool cand = some && make_key(tm, base) > thr;
-    const int c = __syncthreads_count(cand);
-    if (tid == 0 && i + kStages < tiles) fill(i + kStages);
-    if (c == 0) continue;
+    bool cand = some && tm == tm && make_key(tm, base) > thr;
+    if (__syncthreads_count(cand) == 0) {
+      if (tid == 0 && i + kStages < tiles) fill(i + kStages);
+      continue;
+    }
     const int n0 = n;
-    auto push = [&]() {
-      if (!cand) return;
-#pragma unroll
-      for (int u = 0; u < kWords; ++u) {
-        if (tid + u * kThreads < nw) {
-#pragma unroll
-          for (int j = 0; j < kPer; ++j) {
-            const u64 key = make_key(Elem<T>::get(v[u], j), base + u * kThreads * kPer + j);
+    // The logits of the warp's candidate threads, a 32-bit piece of the ring per lane.
+    auto push = [&](int u0, int u1) {
+      for (unsigned int left = __ballot_sync(~0u, cand); left; left &= left - 1) {
+        const int from = __ffs(left) - 1, a = (tid & ~31) + from + (lane >> 2) * kThreads, q = lane & 3;
+        if (a < nw && (lane >> 2) >= u0 && (lane >> 2) < u1) {
+          const unsigned int x = reinterpret_cast<const unsigned int*>(&sh.ring[st][a])[q];
+          const int at = head + (w0 + i * kTileWords + a) * kPer + q * (kPer / 4);
+          auto offer = [&](float f, int idx) {
+            const u64 key = make_key(f, idx);
             if (key > thr) {
-              const int at = atomicAdd(&sh.n, 1);
-              if (at < kList) sh.list[at] = key;
+              const int to = atomicAdd(&sh.n, 1);
+              if (to < kList) sh.list[to] = key;
             }
+          };
+          if constexpr (kPer == 8) {
+            const float2 f = Elem<T>::pair(x);
+            offer(f.x, at);
+            offer(f.y, at + 1);
+          } else {
+            offer(__uint_as_float(x), at);
           }
         }
       }
     };
+    static_assert(kWords == 8, "a candidate's words are one piece per lane");
     if (thr == 0) {
       // No threshold yet: each warp's ceil(k / warps)-th largest thread maximum; the
       // lowest of them is reached by at least k threads' maxima.
@@ -514,110 +625,139 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Param
       for (int j = 0; j < (k + kWarps - 1) / kWarps; ++j) {
         best = __reduce_max_sync(~0u, o);
         const unsigned int who = __ballot_sync(~0u, o == best);
-        if ((tid & 31) == __ffs(who) - 1) o = 0;
+        if (lane == __ffs(who) - 1) o = 0;
       }
-      if ((tid & 31) == 0) sh.warp_key[tid >> 5] = best;
+      if (lane == 0) sh.warp_key[warp] = best;
       __syncthreads();
       u64 low = ~0ull;
 #pragma unroll
       for (int j = 0; j < kWarps; ++j) low = sh.warp_key[j] < low ? sh.warp_key[j] : low;
       if (low) {
         thr = (low << 32) - 1;
-        cand = some && make_key(tm, base) > thr;
+        cand = cand && make_key(tm, base) > thr;
       }
     }
-    push();
+    push(0, kWords);
     __syncthreads();
     n = sh.n;
     if (n > kList) {
-      // More than the list holds (equal or rising logits): drop this tile's, lower the
-      // list to kKeep, and take a threshold that at most kMaxTop threads reach.
+      // More than the list holds (equal or rising logits): drop this tile's, shorten the
+      // list, and take a threshold that at most kMaxTop threads reach.
       __syncthreads();
       if (tid == 0) sh.n = n0;
       __syncthreads();
       n = n0;
-      if (n0 > kKeep) {
-        const u64 t = prune(sh, n0, k, turn);
-        thr = t > thr ? t : thr;
-        n = sh.n;
+      if (n0 > k) {
+        thr = prune(sh, n0, k, turn);
+        n = k;
       }
       u64 best = 0;  // the thread's largest key
-      if (some) {
-#pragma unroll
-        for (int u = kWords - 1; u >= 0; --u)
-#pragma unroll
-          for (int j = kPer - 1; j >= 0; --j) {
-            const u64 key = make_key(Elem<T>::get(v[u], j), base + u * kThreads * kPer + j);
-            if (tid + u * kThreads < nw && key > best) best = key;
-          }
-      }
-      int over = block_count(sh, best > thr, turn);
-      if (over > kMaxTop) {
-        thr = search(sh, turn, thr, k, kMaxTop, 1, [&](int) { return best; });
-      }
-      cand = best > thr;
-      __syncthreads();
-      push();
-      __syncthreads();
-      n = sh.n;
-    }
-    if (n > kPruneAt) {
-      const u64 t = prune(sh, n, k, turn);
-      thr = t > thr ? t : thr;
-      n = sh.n;
-    }
-  }
-
-  // ---- this CTA's sums about its maximum
-  {
-    float M = m;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, o));
-    if ((tid & 31) == 0) sh.warp_f[0][tid >> 5] = M;
-    if (tid == 0) sh.owner = kThreads;
-    __syncthreads();
-    M = sh.warp_f[0][0];
-#pragma unroll
-    for (int i = 1; i < kWarps; ++i) M = fmaxf(M, sh.warp_f[0][i]);
-    if (m == M && M != neg_inf()) atomicMin(&sh.owner, tid);
-    __syncthreads();
-    if (sh.owner == tid) {
-      // Sum the tile that holds the maximum again, without it.
-      float rest = p_ref != p_ref ? p_ref : 0.f;
-      if (ref_tile >= 0) {
-        bool left_out = false;
-        for (int u = 0; u < kWords; ++u) {
-          const int a = ref_tile * kTileWords + tid + u * kThreads;
-          if (a >= w1 - w0) break;
-          const uint4 word = __ldg(xw + a);
-#pragma unroll
+      for (int u = 0; u < kWords; ++u) {
+        const int a = tid + u * kThreads;
+        if (a < nw) {
           for (int j = 0; j < kPer; ++j) {
-            const float f = Elem<T>::get(word, j);
-            if (!left_out && f == M) left_out = true;
-            else rest += fast_exp2(max_nan((f - M) * kLog2e, -200.f));
+            const u64 key = make_key(Elem<T>::load(sh.ring[st], (long long)a * kPer + j),
+                                     head + (w0 + i * kTileWords + a) * kPer + j);
+            best = key > best ? key : best;
           }
         }
       }
-      p_ref = rest;
+      if (block_count(sh, best > thr, turn) > kMaxTop)
+        thr = search(sh, turn, thr, k, kMaxTop, 1, [&](int) { return best; });
+      for (int u = 0; u < kWords; u += kRound) {
+        cand = best > thr;
+        push(u, u + kRound);
+        __syncthreads();
+        n = sh.n;
+        if (n > k) {
+          thr = prune(sh, n, k, turn);
+          n = k;
+        } else {
+          __syncthreads();
+        }
+      }
     }
-    const float dt = step_down(m, M), f = fast_exp2(dt), all = s + p_ref;
-    const float r = warp_sum(f * all), q = warp_sum(f * fmaf(all, dt, w));
+    if (n > k + kPruneAt) {
+      thr = prune(sh, n, k, turn);
+      n = k;
+    }
+    if (tid == 0 && i + kStages < tiles) fill(i + kStages);
+  }
+  flush();
+
+  // ---- this CTA's sums about its maximum
+  {
+    if (lane == 0) sh.warp_f[0][warp] = m;
+    __syncthreads();
+    float M = sh.warp_f[0][0];
+    int owner = 0;
+#pragma unroll
+    for (int i = 1; i < kWarps; ++i) {
+      const float other = sh.warp_f[0][i];
+      owner = other > M ? i : owner;
+      M = fmaxf(M, other);
+    }
+    if (owner == warp && M != neg_inf()) {
+      // Sum the tile that holds the maximum again, without it.
+      const float keep = p_ref != p_ref ? p_ref : 0.f;
+      float rest = keep;
+      int mine = 0;  // logits equal to the maximum
+      if (ref_tile < 0) {
+        mine = lone == M;
+        if (!mine && !(lone < kLow)) rest += fast_exp2(exponent(fmaxf(lone, m - 100.f), mc));
+      } else {
+        const int first = ref_tile * kTileWords + tid;
+        auto take = [&](float f) {
+          if (f == M) ++mine;
+          else rest += fast_exp2(exponent(fmaxf(f, m - 100.f), mc));
+        };
+#pragma unroll
+        for (int u = 0; u < kWords; ++u) {
+          if (first + u * kThreads < w1 - w0) {
+            const uint4 word = __ldg(xw + first + u * kThreads);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              if constexpr (kPer == 8) {
+                const float2 f = Elem<T>::pair(piece(word, q));
+                take(f.x);
+                take(f.y);
+              } else {
+                take(__uint_as_float(piece(word, q)));
+              }
+            }
+          }
+        }
+      }
+      const unsigned int who = __ballot_sync(~0u, mine > 0);
+      const float e0 = fast_exp2(exponent(m, mc));
+      if (lane == __ffs(who) - 1) --mine;
+      p_ref = fmaf((float)mine, e0, rest);
+    }
+    // From the rounded reference to m, then to the CTA's maximum.  The maximum itself, left out of the owner's
+    // sum, has a term in w: e0 t0.
+    const float t0 = m == neg_inf() ? 0.f : exponent(m, mc), inv = fast_exp2(-t0);
+    const float all = s + p_ref, q = (w - t0 * (all + (owner == warp && lane == 0 ? fast_exp2(t0) : 0.f))) * inv;
+    const float dt = bounded((m - M) * kLog2e), f = fast_exp2(dt);
+    const float r_sum = warp_sum(f * inv * all), w_sum = warp_sum(f * fmaf(inv * all, dt, q));
     const int up = __reduce_add_sync(~0u, above);
-    const bool gave_up = __any_sync(~0u, late);
-    if ((tid & 31) == 0) {
-      sh.warp_f[1][tid >> 5] = r;
-      sh.warp_f[2][tid >> 5] = q;
-      sh.warp_above[tid >> 5] = up;
-      if (gave_up && p.error_bits) atomicOr(p.error_bits, kErrTimeout);
+    if (lane == 0) {
+      sh.warp_f[1][warp] = r_sum;
+      sh.warp_f[2][warp] = w_sum;
+      sh.warp_above[warp] = up | (skipped ? kSkipped : 0);
     }
-    if (k) sort_top(sh, n, k, turn);  // (its barriers also order the sums)
-    else __syncthreads();
+    if (__any_sync(~0u, late) && lane == 0 && p.error_bits) atomicOr(p.error_bits, kErrTimeout);
+    if (k) {
+      if (n > kThreads) n = shorten(sh, n, k, turn);
+      rank_list(sh, n, k);  // (its barrier also orders the sums)
+    } else {
+      __syncthreads();
+    }
     Part mine{M, 0.f, 0.f, 0};
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) {
       mine.r += sh.warp_f[1][i];
       mine.w += sh.warp_f[2][i];
-      mine.above += sh.warp_above[i];
+      mine.above = ((mine.above + sh.warp_above[i]) & INT_MAX) | ((mine.above | sh.warp_above[i]) & kSkipped);
     }
     if (splits == 1) {
       if (tid == 0) sh.parts[0] = mine;
@@ -644,7 +784,9 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Param
           if (key) sh.list[atomicAdd(&sh.n, 1)] = key;
         }
         __syncthreads();
-        sort_top(sh, sh.n, k, turn);
+        n = sh.n;
+        if (n > kThreads) n = shorten(sh, n, k, turn);
+        rank_list(sh, n, k);
       }
     }
     __syncthreads();
@@ -653,10 +795,12 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Param
   // ---- the row
   Part a = sh.parts[0];
   for (int i = 1; i < splits; ++i) a = join(a, sh.parts[i]);
-  if (a.r != a.r || a.w != a.w) {
-    unordered_row<T>(sh, p, x, row, tok);
+  if (a.r != a.r || a.w != a.w || a.m > kHighRow ||
+      ((a.above & kSkipped) && !(a.m > kLowRow))) {
+    general_row<T>(sh, p, x, row, tok);
     return;
   }
+  a.above &= INT_MAX;
   const float nan = __int_as_float(0x7fffffff);
   const float ln_s = a.m == neg_inf() ? nan : log1pf(a.r);
   if (tid == 0) {
