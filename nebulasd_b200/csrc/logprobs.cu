@@ -36,6 +36,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kWords = 8;                          // 16-byte words per thread and tile
 constexpr int kTileWords = kThreads * kWords;      // 32 KB
 constexpr int kStages = 2;
+constexpr int kCtas = 3;                            // resident per SM
 constexpr int kMaxTop = NEB_MAX_TOP_LOGPROBS;
 constexpr int kMaxSplits = 8;                      // CTAs per row (the portable cluster size)
 constexpr int kPruneAt = 16;                       // candidates beyond num_top from which a prune pays
@@ -43,7 +44,8 @@ constexpr int kRound = 2;                          // words of a thread that an 
 constexpr int kList = kMaxTop + kPruneAt + kMaxTop * kRound * 8;  // and those of kMaxTop threads
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr long long kWaitLimit = 4000000000ll;     // cycles (about 2 s)
+constexpr uint32_t kWaitNs = 20000;                // a tile's wait: kWaitTries times this, 2 s
+constexpr int kWaitTries = 100000;
 
 typedef unsigned long long u64;
 
@@ -192,11 +194,6 @@ __device__ __forceinline__ u64 add2(u64 a, u64 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
-  u64 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
   u64 r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
@@ -217,7 +214,7 @@ __device__ __forceinline__ float warp_max_nan(float v) {
 __device__ __forceinline__ float exponent(float x, float mc) { return fmaf(x, kLog2e, -mc); }
 
 // Adds a tile's terms 2^t and 2^t t, two fp32 lanes per instruction.  Logits far below the reference count
-// as 100 below it: 2^t is 0 all the same, and 0 times -inf is kept out of the second one.
+// as 100 below it: 2^t is 0 all the same, and 0 times -inf is kept out of the second sum.
 template <typename T>
 __device__ __forceinline__ void add_tile(const uint4 (&v)[kWords], float m, float mc, u64 (&s)[2], u64 (&w)[2]) {
   const u64 c2 = pack2(kLog2e, kLog2e), mc2 = pack2(-mc, -mc);
@@ -283,6 +280,13 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                    sm100::smem_u32(dst)),
                "l"(src), "r"(bytes), "r"(sm100::smem_u32(bar))
                : "memory");
+}
+
+// Bounded (about 2 s), asleep between tries: the other CTAs' warps need the issue slots.
+__device__ __forceinline__ bool wait_full(uint64_t* bar, uint32_t parity) {
+  for (int i = 0; i < kWaitTries; ++i)
+    if (sm100::mbar_try_wait_sleep(bar, parity, kWaitNs)) return true;
+  return false;
 }
 
 // ------------------------------------------------------------ block reductions
@@ -461,7 +465,7 @@ __device__ __noinline__ void general_row(Shared& sh, const Params& p, const void
 
 // --------------------------------------------------------------------- kernel
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const Params p) {
   extern __shared__ __align__(128) unsigned char smem_raw[];
   Shared& sh = *reinterpret_cast<Shared*>(smem_raw);
   constexpr int kPer = Elem<T>::kPerWord;
@@ -509,7 +513,15 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Param
   int ref_tile = -1;  // (-1: the head and tail logits)
   int above = 0;
   bool skipped = false;
-  u64 thr = 0;        // the k-th largest candidate (0: not known yet)
+  // At least k listed logits are thr or above (0: not known yet); its parts, for a quick test.
+  u64 thr = 0;
+  float thr_value = neg_inf();
+  unsigned int thr_index = ~0u;
+  auto set_threshold = [&](u64 key) {
+    thr = key;
+    thr_value = key_value(key);
+    thr_index = ~(unsigned int)key;
+  };
   int n = k && part == 0 ? head + tail : 0;  // candidates listed
   int turn = 0;
   auto flush = [&]() {
@@ -555,13 +567,18 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Param
   for (int i = 0; i < tiles; ++i) {
     const int st = i % kStages;
     const int nw = w1 - w0 - i * kTileWords;  // words from this tile on
-    if (!sm100::mbar_wait(&sh.full[st], (i / kStages) & 1, kWaitLimit)) late = true;
+    if (!wait_full(&sh.full[st], (i / kStages) & 1)) late = true;
     uint4 v[kWords];
+    if (nw >= kTileWords) {
 #pragma unroll
-    for (int u = 0; u < kWords; ++u) {
-      const int a = tid + u * kThreads;
-      v[u] = a < nw ? sh.ring[st][a]
-                    : make_uint4(Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest);
+      for (int u = 0; u < kWords; ++u) v[u] = sh.ring[st][tid + u * kThreads];
+    } else {
+#pragma unroll
+      for (int u = 0; u < kWords; ++u) {
+        const int a = tid + u * kThreads;
+        v[u] = a < nw ? sh.ring[st][a]
+                      : make_uint4(Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest);
+      }
     }
     const float tm = words_max<T>(v), top = warp_max_nan(tm);
     const bool raise = top > m && top >= kLow;
@@ -569,35 +586,16 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Param
       flush();
       raise_to(top, i);
     }
-    // A tile far below the reference (banned tokens) adds nothing.
-    if (top >= m - 120.f) add_tile<T>(v, m, mc, acc_s, acc_w);
-    if (top != top) s = top;
-    else if (m == neg_inf() && top > neg_inf()) skipped = true;
-    if (raise) {
-      const float2 a = unpack2(add2(acc_s[0], acc_s[1]));
-      p_ref = a.x + a.y;
-      acc_s[0] = acc_s[1] = 0;
-    }
-    if (top > given) above += count_above<T>(v, given);
-    if (k == 0) {
-      __syncthreads();  // the ring slot is read
-      if (tid == 0 && i + kStages < tiles) fill(i + kStages);
-      continue;
-    }
     // ---- candidates
     const int base = head + (w0 + i * kTileWords + tid) * kPer;  // index of the thread's first logit
     const bool some = tid < nw;
-    bool cand = some && tm == tm && make_key(tm, base) > thr;
-    if (__syncthreads_count(cand) == 0) {
-      if (tid == 0 && i + kStages < tiles) fill(i + kStages);
-      continue;
-    }
+    bool cand = k && some && (tm > thr_value || (tm == thr_value && (unsigned int)base < thr_index));
     const int n0 = n;
     // The logits of the warp's candidate threads, a 32-bit piece of the ring per lane.
     auto push = [&](int u0, int u1) {
       for (unsigned int left = __ballot_sync(~0u, cand); left; left &= left - 1) {
-        const int from = __ffs(left) - 1, a = (tid & ~31) + from + (lane >> 2) * kThreads, q = lane & 3;
-        if (a < nw && (lane >> 2) >= u0 && (lane >> 2) < u1) {
+        const int from = __ffs(left) - 1, u = lane >> 2, q = lane & 3, a = (tid & ~31) + from + u * kThreads;
+        if (a < nw && u >= u0 && u < u1) {
           const unsigned int x = reinterpret_cast<const unsigned int*>(&sh.ring[st][a])[q];
           const int at = head + (w0 + i * kTileWords + a) * kPer + q * (kPer / 4);
           auto offer = [&](float f, int idx) {
@@ -617,8 +615,9 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Param
         }
       }
     };
-    static_assert(kWords == 8, "a candidate's words are one piece per lane");
-    if (thr == 0) {
+    static_assert(kWords <= 8, "a candidate's words are one piece per lane");
+    if (k && thr == 0) {
+      cand = some && tm == tm;
       // No threshold yet: each warp's ceil(k / warps)-th largest thread maximum; the
       // lowest of them is reached by at least k threads' maxima.
       unsigned int o = some ? order_f32(tm) : 0u, best = 0;
@@ -634,52 +633,66 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Param
       for (int j = 0; j < kWarps; ++j) low = sh.warp_key[j] < low ? sh.warp_key[j] : low;
       if (low) {
         thr = (low << 32) - 1;
+        thr_value = value_of_order((unsigned int)low);
+        thr_index = ~0u;
         cand = cand && make_key(tm, base) > thr;
       }
     }
     push(0, kWords);
-    __syncthreads();
-    n = sh.n;
-    if (n > kList) {
-      // More than the list holds (equal or rising logits): drop this tile's, shorten the
-      // list, and take a threshold that at most kMaxTop threads reach.
+    // A tile far below the reference (banned tokens) adds nothing.
+    if (top >= m - 120.f) add_tile<T>(v, m, mc, acc_s, acc_w);
+    if (top != top) s = top;
+    else if (m == neg_inf() && top > neg_inf()) skipped = true;
+    if (raise) {
+      const float2 a = unpack2(add2(acc_s[0], acc_s[1]));
+      p_ref = a.x + a.y;
+      acc_s[0] = acc_s[1] = 0;
+    }
+    if (top > given) above += count_above<T>(v, given);
+    // The ring slot is read, the tile's candidates are listed.
+    if (__syncthreads_or(cand)) {
+      n = sh.n;
       __syncthreads();
-      if (tid == 0) sh.n = n0;
-      __syncthreads();
-      n = n0;
-      if (n0 > k) {
-        thr = prune(sh, n0, k, turn);
-        n = k;
-      }
-      u64 best = 0;  // the thread's largest key
-      for (int u = 0; u < kWords; ++u) {
-        const int a = tid + u * kThreads;
-        if (a < nw) {
-          for (int j = 0; j < kPer; ++j) {
-            const u64 key = make_key(Elem<T>::load(sh.ring[st], (long long)a * kPer + j),
-                                     head + (w0 + i * kTileWords + a) * kPer + j);
-            best = key > best ? key : best;
+      if (n > kList) {
+        // More than the list holds (equal or rising logits): drop this tile's, shorten the
+        // list, and take a threshold that at most kMaxTop threads reach.
+        if (tid == 0) sh.n = n0;
+        __syncthreads();
+        n = n0;
+        if (n0 > k) {
+          set_threshold(prune(sh, n0, k, turn));
+          n = k;
+        }
+        u64 best = 0;  // the thread's largest key
+        for (int u = 0; u < kWords; ++u) {
+          const int a = tid + u * kThreads;
+          if (a < nw) {
+            for (int j = 0; j < kPer; ++j) {
+              const u64 key = make_key(Elem<T>::load(sh.ring[st], (long long)a * kPer + j),
+                                       head + (w0 + i * kTileWords + a) * kPer + j);
+              best = key > best ? key : best;
+            }
+          }
+        }
+        if (block_count(sh, best > thr, turn) > kMaxTop)
+          set_threshold(search(sh, turn, thr, k, kMaxTop, 1, [&](int) { return best; }));
+        for (int u = 0; u < kWords; u += kRound) {
+          cand = best > thr;
+          push(u, u + kRound);
+          __syncthreads();
+          n = sh.n;
+          if (n > k) {
+            set_threshold(prune(sh, n, k, turn));
+            n = k;
+          } else {
+            __syncthreads();
           }
         }
       }
-      if (block_count(sh, best > thr, turn) > kMaxTop)
-        thr = search(sh, turn, thr, k, kMaxTop, 1, [&](int) { return best; });
-      for (int u = 0; u < kWords; u += kRound) {
-        cand = best > thr;
-        push(u, u + kRound);
-        __syncthreads();
-        n = sh.n;
-        if (n > k) {
-          thr = prune(sh, n, k, turn);
-          n = k;
-        } else {
-          __syncthreads();
-        }
+      if (n > k + kPruneAt) {
+        set_threshold(prune(sh, n, k, turn));
+        n = k;
       }
-    }
-    if (n > k + kPruneAt) {
-      thr = prune(sh, n, k, turn);
-      n = k;
     }
     if (tid == 0 && i + kStages < tiles) fill(i + kStages);
   }
@@ -820,7 +833,7 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Param
 static int choose_splits(long long rows, int vocab, int item, int sms) {
   const long long tiles = ((long long)vocab * item + 16 * kTileWords - 1) / (16 * kTileWords);
   int s = 1;
-  while (s < kMaxSplits && 2 * s <= tiles && rows * s * 2 <= 3ll * sms) s *= 2;
+  while (s < kMaxSplits && 2 * s <= tiles && rows * s * 2 <= (long long)kCtas * sms) s *= 2;
   return s;
 }
 
