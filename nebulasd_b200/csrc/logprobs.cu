@@ -17,11 +17,12 @@
 // their sums and candidates in the first CTA's shared memory, so there is no
 // workspace and no second launch.
 //
-// Alternatives: a CTA keeps a list of candidates and a threshold, the num_top-th
-// of them.  A thread compares its tile maximum (needed for m anyway) with the
-// threshold, and only where it is higher does the warp look at that thread's
-// logits again, in the ring.  So after the first tile a tile costs its barrier and
-// a few candidates.
+// Alternatives: a CTA keeps a list of candidates and a threshold that num_top of
+// them reach.  A lane compares its tile maximum (needed for m anyway) with the
+// threshold, and only where it is higher does the warp look at that lane's logits
+// again, in the ring, and list those above it.  The warp that lists every 8th (16th,
+// 32nd: by num_top) candidate raises the threshold.  So after the first tile a tile costs one
+// comparison and now and then a candidate, and no barrier.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -33,15 +34,14 @@ namespace logprobs {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kWords = 8;                          // 16-byte words per thread and tile
-constexpr int kTileWords = kThreads * kWords;      // 32 KB
+constexpr int kWords = 8;                  // 16-byte words per lane and tile
+constexpr int kTileWords = 32 * kWords;    // of one warp: 4 KB
 constexpr int kStages = 2;
-constexpr int kCtas = 3;                            // resident per SM
+constexpr int kCtas = 3;                   // resident per SM
 constexpr int kMaxTop = NEB_MAX_TOP_LOGPROBS;
-constexpr int kMaxSplits = 8;                      // CTAs per row (the portable cluster size)
-constexpr int kPruneAt = 16;                       // candidates beyond num_top from which a prune pays
-constexpr int kRound = 2;                          // words of a thread that an overfull tile lists at a time
-constexpr int kList = kMaxTop + kPruneAt + kMaxTop * kRound * 8;  // and those of kMaxTop threads
+constexpr int kMaxSplits = 8;              // CTAs per row (the portable cluster size)
+constexpr int kList = 512;                 // candidates
+constexpr int kWindow = 128;               // the last candidates, among which it is looked for
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr uint32_t kWaitNs = 20000;                // a tile's wait: kWaitTries times this, 2 s
@@ -70,16 +70,18 @@ struct Part {
 constexpr int kSkipped = INT_MIN;  // a tile below kLow was left out
 
 struct Shared {
-  uint4 ring[kStages][kTileWords];
+  uint4 ring[kWarps][kStages][kTileWords];
   u64 list[kList];
   u64 sorted[kMaxTop];
   Part parts[kMaxSplits];
   u64 gathered[kMaxSplits][kMaxTop];
-  uint64_t full[kStages];
+  uint64_t full[kWarps][kStages];
   u64 warp_key[kWarps];
+  unsigned int tops[64];
+  u64 threshold;  // only larger keys are listed; num_top listed ones are at or above it
   float warp_f[3][kWarps];
   int warp_count[2][kWarps], warp_above[kWarps];
-  int n;
+  int n;  // candidates offered (beyond kList: not all are listed)
 };
 
 // ------------------------------------------------------------------- elements
@@ -334,12 +336,11 @@ __device__ __forceinline__ u64 search(Shared& sh, int& turn, u64 lo, int lowest,
   return lo;
 }
 
-// The list's num_top largest keys in order (0 where there are fewer) into sh.sorted, by counting: n <= kThreads.
+// The list's num_top largest keys in order (0 where there are fewer) into sh.sorted, by counting.
 __device__ __forceinline__ void rank_list(Shared& sh, int n, int num_top) {
-  const int tid = threadIdx.x;
-  if (n < num_top && tid >= n && tid < num_top) sh.sorted[tid] = 0;
-  if (tid < n) {
-    const u64 key = sh.list[tid];
+  for (int i = threadIdx.x + n; i < num_top; i += kThreads) sh.sorted[i] = 0;
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const u64 key = sh.list[i];
     int before = 0;
     for (int j = 0; j < n; ++j) before += sh.list[j] > key;
     if (before < num_top) sh.sorted[before] = key;
@@ -347,37 +348,135 @@ __device__ __forceinline__ void rank_list(Shared& sh, int n, int num_top) {
   __syncthreads();
 }
 
-// Shortens a list of n > kThreads candidates to at most kThreads, num_top or more.
-__device__ __noinline__ int shorten(Shared& sh, int n, int num_top, int& turn) {
-  constexpr int kEach = (kList + kThreads - 1) / kThreads;
-  u64 key[kEach];
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int at = threadIdx.x + i * kThreads;
-    key[i] = at < n ? sh.list[at] : 0;
+// Lists the logits above the threshold among the words of the warp's candidate lanes, a 32-bit piece of the
+// tile per lane.  `first`: the index of the tile's first logit, `value` the threshold's.  True when it is time for
+// a better threshold: after every `every`-th candidate (a power of two).
+template <typename T>
+__device__ __forceinline__ bool list_candidates(Shared& sh, const uint4* tile, int words, int first, bool cand,
+                                                float value, int every) {
+  constexpr int kPer = Elem<T>::kPerWord;
+  static_assert(kWords * 4 == 32, "a lane's words are one piece per lane");
+  const int lane = threadIdx.x & 31, word = (lane >> 2) * 32;
+  const unsigned int* piece_of = reinterpret_cast<const unsigned int*>(tile + word) + (lane & 3);
+  bool due = false;
+  auto offer = [&](float f, int idx) {
+    const u64 key = make_key(f, idx);
+    if (key > *static_cast<volatile u64*>(&sh.threshold)) {
+      const int to = atomicAdd(&sh.n, 1);
+      if (to < kList) sh.list[to] = key;
+      due |= ((to + 1) & (every - 1)) == 0;
+    }
+  };
+  if (*static_cast<volatile int*>(&sh.n) > kList) return false;
+  for (unsigned int left = __ballot_sync(~0u, cand); left; left &= left - 1) {
+    const int from = __ffs(left) - 1;
+    if (from + word < words) {
+      const unsigned int x = piece_of[4 * from];
+      const int at = first + (from + word) * kPer + (lane & 3) * (kPer / 4);
+      if constexpr (kPer == 8) {
+        const float2 f = Elem<T>::pair(x);
+        if (f.x >= value) offer(f.x, at);
+        if (f.y >= value) offer(f.y, at + 1);
+      } else {
+        if (__uint_as_float(x) >= value) offer(__uint_as_float(x), at);
+      }
+    }
   }
-  const u64 thr = search(sh, turn, 0, num_top, kThreads, kEach, [&](int i) { return key[i]; });
-  __syncthreads();
-  if (threadIdx.x == 0) sh.n = 0;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kEach; ++i)
-    if (key[i] > thr) sh.list[atomicAdd(&sh.n, 1)] = key[i];
-  __syncthreads();
-  n = sh.n;
+  return __any_sync(~0u, due);
+}
+
+// Raises the threshold to the num_top-th largest of the last candidates, by one warp.  Others may be listing
+// meanwhile: a place that is not written yet holds 0, which only makes the threshold lower.
+__device__ __noinline__ void raise_threshold(Shared& sh, int num_top) {
+  const int n = min(*static_cast<volatile int*>(&sh.n), kList), from = max(0, n - kWindow);
+  for (int i = from + (threadIdx.x & 31); i < n; i += 32) {
+    const u64 key = sh.list[i];
+    int before = 0;
+#pragma unroll 4
+    for (int j = from; j < n; ++j) before += sh.list[j] > key;
+    if (key && before == num_top - 1) atomicMax(&sh.threshold, key);
+  }
+}
+
+// The candidates of a row part whose list ran over (equal or rising logits), word by word from memory: the
+// num_top largest, in sh.list.  Returns how many.
+template <typename T>
+__device__ __noinline__ int collect(Shared& sh, const uint4* data, int words, int first, const void* x, int vocab,
+                                    int head, int tail, int k) {
+  constexpr int kPer = Elem<T>::kPerWord;
+  constexpr int kMost = kThreads - kMaxTop;
+  const int tid = threadIdx.x;
+  int turn = 0, n = 0;
+  u64 thr = ((u64)order_f32(kLow) << 32) - 1;
+  for (int base = 0; base == 0 || base < words; base += kThreads) {
+    u64 key[kPer + 1] = {};
+    if (base + tid < words) {
+      for (int j = 0; j < kPer; ++j) {
+        const long long at = (long long)(base + tid) * kPer + j;
+        key[j] = make_key(Elem<T>::load(data, at), first + (int)at);
+      }
+    }
+    if (base == 0 && tid < head + tail) {
+      const int at = tid < head ? tid : vocab - tail + (tid - head);
+      key[kPer] = make_key(Elem<T>::load(x, at), at);
+    }
+    int c = 0;
+    for (int j = 0; j <= kPer; ++j) c += key[j] > thr;
+    c = block_count(sh, c, turn);
+    if (c == 0) continue;
+    if (c > kMost) thr = search(sh, turn, thr, k, kMost, kPer + 1, [&](int j) { return key[j]; });
+    if (tid == 0) sh.n = n;
+    __syncthreads();
+    for (int j = 0; j <= kPer; ++j)
+      if (key[j] > thr) sh.list[atomicAdd(&sh.n, 1)] = key[j];
+    __syncthreads();
+    n = sh.n;
+    rank_list(sh, n, k);
+    n = min(n, k);
+    if (tid < n) sh.list[tid] = sh.sorted[tid];
+    if (n == k) thr = sh.sorted[k - 1] > thr ? sh.sorted[k - 1] : thr;
+    __syncthreads();
+  }
   return n;
 }
 
-// Leaves the num_top largest of the list's n >= num_top candidates, in order; returns the last of them,
-// which is the threshold from here on.
-__device__ __forceinline__ u64 prune(Shared& sh, int n, int num_top, int& turn) {
-  if (n > kThreads) n = shorten(sh, n, num_top, turn);
-  rank_list(sh, n, num_top);
-  if (threadIdx.x < num_top) sh.list[threadIdx.x] = sh.sorted[threadIdx.x];
-  if (threadIdx.x == 0) sh.n = num_top;
-  const u64 last = sh.sorted[num_top - 1];
+// Fills sh.sorted from n to k with the logits below kLow, which the candidates leave out: largest first (all of
+// them mostly equal, -inf or another mask), then by index.
+template <typename T>
+__device__ __noinline__ void fill_masked(Shared& sh, const void* x, int vocab, int n, int k) {
+  const int tid = threadIdx.x;
+  int turn = 0;
+  float limit = kLow;
+  while (n < k) {
+    unsigned int best = 0;
+    for (int j = tid; j < vocab; j += kThreads) {
+      const float v = Elem<T>::load(x, j);
+      if (v < limit) best = max(best, order_f32(v));
+    }
+    best = __reduce_max_sync(~0u, best);
+    __syncthreads();
+    if ((tid & 31) == 0) sh.warp_key[tid >> 5] = best;
+    __syncthreads();
+    for (int i = 0; i < kWarps; ++i) best = max(best, (unsigned int)sh.warp_key[i]);
+    if (best == 0) break;  // (not reached: k is at most the vocabulary)
+    for (int base = 0; base < vocab && n < k; base += kThreads) {
+      const int j = base + tid;
+      const bool hit = j < vocab && order_f32(Elem<T>::load(x, j)) == best;
+      const unsigned int who = __ballot_sync(~0u, hit);
+      if ((tid & 31) == 0) sh.warp_count[turn][tid >> 5] = __popc(who);
+      __syncthreads();
+      int before = __popc(who & ((1u << (tid & 31)) - 1)), all = 0;
+      for (int i = 0; i < kWarps; ++i) {
+        if (i < (tid >> 5)) before += sh.warp_count[turn][i];
+        all += sh.warp_count[turn][i];
+      }
+      turn ^= 1;
+      if (hit && n + before < k) sh.sorted[n + before] = ((u64)best << 32) | (unsigned int)~(unsigned int)j;
+      n += all;
+    }
+    limit = value_of_order(best);
+  }
   __syncthreads();
-  return last;
 }
 
 // Joins `b` into `a`: sums about the larger maximum, which alone is left out of r.
@@ -474,36 +573,36 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const P
   const T* x = static_cast<const T*>(p.logits) + (long long)row * p.row_stride;
   const int k = p.num_top;
 
-  // [head logits][16-byte words][tail logits]
+  // [head logits][16-byte words][tail logits]; the CTA's words go round its warps in tiles.
   const int head = min(p.vocab, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
-  const int words = (p.vocab - head) / kPer;
-  const int tail = p.vocab - head - words * kPer;
-  const int w0 = (int)((long long)words * part / splits), w1 = (int)((long long)words * (part + 1) / splits);
-  const int tiles = (w1 - w0 + kTileWords - 1) / kTileWords;
-  const uint4* xw = reinterpret_cast<const uint4*>(x + head) + w0;
+  const int row_words = (p.vocab - head) / kPer, tail = p.vocab - head - row_words * kPer;
+  const int w0 = (int)((long long)row_words * part / splits);
+  const int words = (int)((long long)row_words * (part + 1) / splits) - w0;
+  const uint4* data = reinterpret_cast<const uint4*>(x + head) + w0;
+  const int tiles = (words + kTileWords - 1) / kTileWords;
+  const int mine = (tiles - warp + kWarps - 1) / kWarps;  // (0 or less: none)
 
-  if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) sm100::mbar_init(&sh.full[i], 1);
-    sm100::fence_mbar_init();
-    sh.n = 0;
-  }
-  auto fill = [&](int tile) {  // by one thread
-    const int st = tile % kStages;
-    const uint32_t bytes = 16u * min(kTileWords, w1 - w0 - tile * kTileWords);
-    sm100::mbar_arrive_expect_tx(&sh.full[st], bytes);
-    bulk_load(sh.ring[st], xw + (long long)tile * kTileWords, bytes, &sh.full[st]);
+  auto fill = [&](int i) {  // the warp's tile i, by one lane
+    const int st = i % kStages, from = (warp + i * kWarps) * kTileWords;
+    const uint32_t bytes = 16u * min(kTileWords, words - from);
+    sm100::mbar_arrive_expect_tx(&sh.full[warp][st], bytes);
+    bulk_load(sh.ring[warp][st], data + from, bytes, &sh.full[warp][st]);
   };
-  if (tid == 0)
-    for (int i = 0; i < min(kStages, tiles); ++i) fill(i);
-  if (splits > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
-
-  int tok = p.token_ids ? p.token_ids[row] : -1;
-  if (tok < -1 || tok >= p.vocab) {
-    if (tid == 0 && part == 0 && p.error_bits) atomicOr(p.error_bits, kErrTokenId);
-    tok = -1;
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i) sm100::mbar_init(&sh.full[warp][i], 1);
+    sm100::fence_mbar_init();
+    for (int i = 0; i < min(kStages, mine); ++i) fill(i);
   }
-  const float given = tok >= 0 ? Elem<T>::load(x, tok) : __int_as_float(0x7f800000);
-  __syncthreads();
+  if (splits > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+  // The token now, its logit once a tile has been waited for: neither load is waited for alone.
+  int tok = p.token_ids ? p.token_ids[row] : -1;
+  float given = __int_as_float(0x7f800000);
+  for (int i = tid; i < kList; i += kThreads) sh.list[i] = 0;
+  if (tid == 0) {
+    sh.n = 0;
+    sh.threshold = ((u64)order_f32(kLow) << 32) - 1;  // masked logits are no candidates
+  }
+  __syncwarp();
 
   // Per warp: the reference m, rounded to mc in base 2.  Per lane: sums of the tiles since the one that
   // holds m (acc_*), of the tiles before it (s, w) and of that tile itself (p_ref), which is kept
@@ -513,17 +612,6 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const P
   int ref_tile = -1;  // (-1: the head and tail logits)
   int above = 0;
   bool skipped = false;
-  // At least k listed logits are thr or above (0: not known yet); its parts, for a quick test.
-  u64 thr = 0;
-  float thr_value = neg_inf();
-  unsigned int thr_index = ~0u;
-  auto set_threshold = [&](u64 key) {
-    thr = key;
-    thr_value = key_value(key);
-    thr_index = ~(unsigned int)key;
-  };
-  int n = k && part == 0 ? head + tail : 0;  // candidates listed
-  int turn = 0;
   auto flush = [&]() {
     const float2 a = unpack2(add2(acc_s[0], acc_s[1])), b = unpack2(add2(acc_w[0], acc_w[1]));
     s += a.x + a.y;
@@ -543,10 +631,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const P
   float lone = neg_inf();  // a lane's head or tail logit
   if (part == 0 && warp == 0) {
     if (lane < head + tail) {
-      const int j = lane < head ? lane : head + words * kPer + (lane - head);
+      const int j = lane < head ? lane : p.vocab - tail + (lane - head);
       lone = Elem<T>::load(x, j);
-      above = lone > given;
-      if (k) sh.list[atomicAdd(&sh.n, 1)] = make_key(lone, j);
     }
     __syncwarp();
     const float top = warp_max_nan(lone != lone ? neg_inf() : lone);
@@ -564,81 +650,81 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const P
   }
 
   bool late = false;
-  for (int i = 0; i < tiles; ++i) {
-    const int st = i % kStages;
-    const int nw = w1 - w0 - i * kTileWords;  // words from this tile on
-    if (!wait_full(&sh.full[st], (i / kStages) & 1)) late = true;
+  const int every = k <= 8 ? 8 : k <= 16 ? 16 : 32;
+  for (int i = 0; i < max(mine, 1); ++i) {
+    const int st = i % kStages, from = (warp + i * kWarps) * kTileWords;
+    const int nw = words - from;  // words from this tile on
+    if (i < mine && !wait_full(&sh.full[warp][st], (i / kStages) & 1)) late = true;
+    if (i == 0) {
+      if (tok >= 0 && tok < p.vocab) {
+        given = Elem<T>::load(x, tok);
+      } else if (tok != -1) {
+        if (tid == 0 && part == 0 && p.error_bits) atomicOr(p.error_bits, kErrTokenId);
+        tok = -1;
+      }
+    }
     uint4 v[kWords];
     if (nw >= kTileWords) {
 #pragma unroll
-      for (int u = 0; u < kWords; ++u) v[u] = sh.ring[st][tid + u * kThreads];
+      for (int u = 0; u < kWords; ++u) v[u] = sh.ring[warp][st][lane + u * 32];
     } else {
 #pragma unroll
       for (int u = 0; u < kWords; ++u) {
-        const int a = tid + u * kThreads;
-        v[u] = a < nw ? sh.ring[st][a]
+        const int a = lane + u * 32;
+        v[u] = a < nw ? sh.ring[warp][st][a]
                       : make_uint4(Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest);
       }
     }
     const float tm = words_max<T>(v), top = warp_max_nan(tm);
+
+    // ---- candidates
+    bool due = false;
+    if (k) {
+      const int first = head + (w0 + from) * kPer;  // index of the tile's first logit
+      if (i == 0) {
+        // The first threshold: the k-th largest of the top lane maxima of each warp whose lanes all have logits.
+        const int whole = words >= 32 ? min(kWarps, (words - 32) / kTileWords + 1) : 0;
+        const int each = whole == kWarps ? min(k, 4) : whole ? (k + whole - 1) / whole : 0;
+        unsigned int o = tm >= kLow ? order_f32(tm) : 0u;
+        if (warp < whole) {
+          for (int j = 0; j < each; ++j) {
+            const unsigned int best = __reduce_max_sync(~0u, o);
+            const unsigned int who = __ballot_sync(~0u, o == best);
+            if (lane == __ffs(who) - 1) {
+              sh.tops[warp * each + j] = best;
+              o = 0;
+            }
+          }
+        }
+        __syncthreads();
+        unsigned int a = lane < whole * each ? sh.tops[lane] : 0u, b = lane + 32 < whole * each ? sh.tops[lane + 32] : 0u;
+        unsigned int low = 0;
+        for (int j = 0; j < k && whole; ++j) {
+          low = __reduce_max_sync(~0u, max(a, b));
+          const unsigned int who = __ballot_sync(~0u, max(a, b) == low);
+          if (lane == __ffs(who) - 1) {
+            if (a == low) a = 0;
+            else b = 0;
+          }
+        }
+        if (low && lane == 0) atomicMax(&sh.threshold, ((u64)low << 32) - 1);
+        __syncwarp();
+        const u64 key = make_key(lone, lane < head ? lane : p.vocab - tail + (lane - head));
+        if (key > *static_cast<volatile u64*>(&sh.threshold)) sh.list[atomicAdd(&sh.n, 1)] = key;
+      }
+      const float thr_value = value_of_order(reinterpret_cast<volatile unsigned int*>(&sh.threshold)[1]);
+      const bool cand = tm >= thr_value;
+      if (__any_sync(~0u, cand)) due = list_candidates<T>(sh, sh.ring[warp][st], nw, first, cand, thr_value, every);
+    }
+    __syncwarp();  // the ring slot is read
+    if (lane == 0 && i + kStages < mine) fill(i + kStages);
+
+    // ---- sums, while the next tiles arrive
     const bool raise = top > m && top >= kLow;
     if (raise) {
       flush();
       raise_to(top, i);
     }
-    // ---- candidates
-    const int base = head + (w0 + i * kTileWords + tid) * kPer;  // index of the thread's first logit
-    const bool some = tid < nw;
-    bool cand = k && some && (tm > thr_value || (tm == thr_value && (unsigned int)base < thr_index));
-    const int n0 = n;
-    // The logits of the warp's candidate threads, a 32-bit piece of the ring per lane.
-    auto push = [&](int u0, int u1) {
-      for (unsigned int left = __ballot_sync(~0u, cand); left; left &= left - 1) {
-        const int from = __ffs(left) - 1, u = lane >> 2, q = lane & 3, a = (tid & ~31) + from + u * kThreads;
-        if (a < nw && u >= u0 && u < u1) {
-          const unsigned int x = reinterpret_cast<const unsigned int*>(&sh.ring[st][a])[q];
-          const int at = head + (w0 + i * kTileWords + a) * kPer + q * (kPer / 4);
-          auto offer = [&](float f, int idx) {
-            const u64 key = make_key(f, idx);
-            if (key > thr) {
-              const int to = atomicAdd(&sh.n, 1);
-              if (to < kList) sh.list[to] = key;
-            }
-          };
-          if constexpr (kPer == 8) {
-            const float2 f = Elem<T>::pair(x);
-            offer(f.x, at);
-            offer(f.y, at + 1);
-          } else {
-            offer(__uint_as_float(x), at);
-          }
-        }
-      }
-    };
-    static_assert(kWords <= 8, "a candidate's words are one piece per lane");
-    if (k && thr == 0) {
-      cand = some && tm == tm;
-      // No threshold yet: each warp's ceil(k / warps)-th largest thread maximum; the
-      // lowest of them is reached by at least k threads' maxima.
-      unsigned int o = some ? order_f32(tm) : 0u, best = 0;
-      for (int j = 0; j < (k + kWarps - 1) / kWarps; ++j) {
-        best = __reduce_max_sync(~0u, o);
-        const unsigned int who = __ballot_sync(~0u, o == best);
-        if (lane == __ffs(who) - 1) o = 0;
-      }
-      if (lane == 0) sh.warp_key[warp] = best;
-      __syncthreads();
-      u64 low = ~0ull;
-#pragma unroll
-      for (int j = 0; j < kWarps; ++j) low = sh.warp_key[j] < low ? sh.warp_key[j] : low;
-      if (low) {
-        thr = (low << 32) - 1;
-        thr_value = value_of_order((unsigned int)low);
-        thr_index = ~0u;
-        cand = cand && make_key(tm, base) > thr;
-      }
-    }
-    push(0, kWords);
     // A tile far below the reference (banned tokens) adds nothing.
     if (top >= m - 120.f) add_tile<T>(v, m, mc, acc_s, acc_w);
     if (top != top) s = top;
@@ -649,54 +735,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const P
       acc_s[0] = acc_s[1] = 0;
     }
     if (top > given) above += count_above<T>(v, given);
-    // The ring slot is read, the tile's candidates are listed.
-    if (__syncthreads_or(cand)) {
-      n = sh.n;
-      __syncthreads();
-      if (n > kList) {
-        // More than the list holds (equal or rising logits): drop this tile's, shorten the
-        // list, and take a threshold that at most kMaxTop threads reach.
-        if (tid == 0) sh.n = n0;
-        __syncthreads();
-        n = n0;
-        if (n0 > k) {
-          set_threshold(prune(sh, n0, k, turn));
-          n = k;
-        }
-        u64 best = 0;  // the thread's largest key
-        for (int u = 0; u < kWords; ++u) {
-          const int a = tid + u * kThreads;
-          if (a < nw) {
-            for (int j = 0; j < kPer; ++j) {
-              const u64 key = make_key(Elem<T>::load(sh.ring[st], (long long)a * kPer + j),
-                                       head + (w0 + i * kTileWords + a) * kPer + j);
-              best = key > best ? key : best;
-            }
-          }
-        }
-        if (block_count(sh, best > thr, turn) > kMaxTop)
-          set_threshold(search(sh, turn, thr, k, kMaxTop, 1, [&](int) { return best; }));
-        for (int u = 0; u < kWords; u += kRound) {
-          cand = best > thr;
-          push(u, u + kRound);
-          __syncthreads();
-          n = sh.n;
-          if (n > k) {
-            set_threshold(prune(sh, n, k, turn));
-            n = k;
-          } else {
-            __syncthreads();
-          }
-        }
-      }
-      if (n > k + kPruneAt) {
-        set_threshold(prune(sh, n, k, turn));
-        n = k;
-      }
-    }
-    if (tid == 0 && i + kStages < tiles) fill(i + kStages);
+    if (due) raise_threshold(sh, k);
   }
   flush();
+  above += lone > given;
 
   // ---- this CTA's sums about its maximum
   {
@@ -719,15 +761,15 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const P
         mine = lone == M;
         if (!mine && !(lone < kLow)) rest += fast_exp2(exponent(fmaxf(lone, m - 100.f), mc));
       } else {
-        const int first = ref_tile * kTileWords + tid;
+        const int first = (warp + ref_tile * kWarps) * kTileWords + lane;
         auto take = [&](float f) {
           if (f == M) ++mine;
           else rest += fast_exp2(exponent(fmaxf(f, m - 100.f), mc));
         };
-#pragma unroll
+#pragma unroll 1
         for (int u = 0; u < kWords; ++u) {
-          if (first + u * kThreads < w1 - w0) {
-            const uint4 word = __ldg(xw + first + u * kThreads);
+          if (first + u * 32 < words) {
+            const uint4 word = __ldg(data + first + u * 32);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
               if constexpr (kPer == 8) {
@@ -759,11 +801,11 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const P
       sh.warp_above[warp] = up | (skipped ? kSkipped : 0);
     }
     if (__any_sync(~0u, late) && lane == 0 && p.error_bits) atomicOr(p.error_bits, kErrTimeout);
+    __syncthreads();
     if (k) {
-      if (n > kThreads) n = shorten(sh, n, k, turn);
-      rank_list(sh, n, k);  // (its barrier also orders the sums)
-    } else {
-      __syncthreads();
+      int n = sh.n;
+      if (n > kList) n = collect<T>(sh, data, words, head + w0 * kPer, x, p.vocab, part ? 0 : head, part ? 0 : tail, k);
+      rank_list(sh, n, k);
     }
     Part mine{M, 0.f, 0.f, 0};
 #pragma unroll
@@ -797,9 +839,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const P
           if (key) sh.list[atomicAdd(&sh.n, 1)] = key;
         }
         __syncthreads();
-        n = sh.n;
-        if (n > kThreads) n = shorten(sh, n, k, turn);
-        rank_list(sh, n, k);
+        rank_list(sh, sh.n, k);
       }
     }
     __syncthreads();
@@ -814,6 +854,12 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const P
     return;
   }
   a.above &= INT_MAX;
+  if (k && sh.sorted[k - 1] == 0) {
+    int listed = 0;
+    while (sh.sorted[listed]) ++listed;
+    __syncthreads();
+    fill_masked<T>(sh, x, p.vocab, listed, k);
+  }
   const float nan = __int_as_float(0x7fffffff);
   const float ln_s = a.m == neg_inf() ? nan : log1pf(a.r);
   if (tid == 0) {
