@@ -11,16 +11,16 @@
 // confident row has log p = -log1p(r) with r << 1, which 1 + r would round away.
 //
 // A row is streamed by a cluster of S CTAs (S = 1 when the rows alone fill the
-// GPU), each through a ring of 32 KB tiles filled by bulk asynchronous copies
-// while the tiles before are summed from registers: the row is read once, the
-// ring keeps the loads in flight whatever the arithmetic does.  The CTAs leave
+// GPU), each warp through a 4 KB tile of shared memory that a bulk asynchronous
+// copy fills while the tile before is summed from registers.  No warp waits for
+// another, and the row is read once.  The CTAs leave
 // their sums and candidates in the first CTA's shared memory, so there is no
 // workspace and no second launch.
 //
 // Alternatives: a CTA keeps a list of candidates and a threshold that num_top of
 // them reach.  A lane compares its tile maximum (needed for m anyway) with the
 // threshold, and only where it is higher does the warp look at that lane's logits
-// again, in the ring, and list those above it.  The warp that lists every 8th (16th,
+// again, in the tile, and list those above it.  The warp that lists every 8th (16th,
 // 32nd: by num_top) candidate raises the threshold.  So after the first tile a tile costs one
 // comparison and now and then a candidate, and no barrier.
 #include <cuda_bf16.h>
@@ -36,8 +36,7 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kWords = 8;                  // 16-byte words per lane and tile
 constexpr int kTileWords = 32 * kWords;    // of one warp: 4 KB
-constexpr int kStages = 2;
-constexpr int kCtas = 3;                   // resident per SM
+constexpr int kCtas = 4;                   // resident per SM
 constexpr int kMaxTop = NEB_MAX_TOP_LOGPROBS;
 constexpr int kMaxSplits = 8;              // CTAs per row (the portable cluster size)
 constexpr int kList = 512;                 // candidates
@@ -70,12 +69,12 @@ struct Part {
 constexpr int kSkipped = INT_MIN;  // a tile below kLow was left out
 
 struct Shared {
-  uint4 ring[kWarps][kStages][kTileWords];
+  uint4 slot[kWarps][kTileWords];
   u64 list[kList];
   u64 sorted[kMaxTop];
   Part parts[kMaxSplits];
   u64 gathered[kMaxSplits][kMaxTop];
-  uint64_t full[kWarps][kStages];
+  uint64_t full[kWarps];
   u64 warp_key[kWarps];
   unsigned int tops[64];
   u64 threshold;  // only larger keys are listed; num_top listed ones are at or above it
@@ -215,24 +214,30 @@ __device__ __forceinline__ float warp_max_nan(float v) {
 // itself is t0, not 0; e0 = 2^t0 takes that out of the finished sums.
 __device__ __forceinline__ float exponent(float x, float mc) { return fmaf(x, kLog2e, -mc); }
 
-// Adds a tile's terms 2^t and 2^t t, two fp32 lanes per instruction.  Logits far below the reference count
-// as 100 below it: 2^t is 0 all the same, and 0 times -inf is kept out of the second sum.
+// Where logits far below the reference are cut off: their terms are 0 all the same.
 template <typename T>
-__device__ __forceinline__ void add_tile(const uint4 (&v)[kWords], float m, float mc, u64 (&s)[2], u64 (&w)[2]) {
+__device__ __forceinline__ float low_end(float m) {
+  return fmaxf(m - 100.f - fabsf(m) * Elem<T>::kUlp, kFinite);
+}
+
+// Adds a tile's terms 2^t and 2^t t, two fp32 lanes per instruction.  The cut-off keeps
+// 0 times -inf out of the second sum.
+template <typename T>
+__device__ __forceinline__ void add_tile(const uint4 (&v)[kWords], float m, float mc, u64& s, u64& w) {
   const u64 c2 = pack2(kLog2e, kLog2e), mc2 = pack2(-mc, -mc);
-  const float lo = fmaxf(m - 100.f - fabsf(m) * Elem<T>::kUlp, kFinite);
-  auto add = [&](float a, float b, int i) {
+  const float lo = low_end<T>(m);
+  auto add = [&](float a, float b) {
     const u64 t = fma2(pack2(a, b), c2, mc2);
     const float2 f = unpack2(t);
     const u64 e = pack2(fast_exp2(f.x), fast_exp2(f.y));
-    s[i] = add2(s[i], e);
-    w[i] = fma2(e, t, w[i]);
+    s = add2(s, e);
+    w = fma2(e, t, w);
   };
   if constexpr (Elem<T>::kPerWord == 4) {
 #pragma unroll
     for (int u = 0; u < kWords; ++u) {
-      add(fmaxf(__uint_as_float(v[u].x), lo), fmaxf(__uint_as_float(v[u].y), lo), 0);
-      add(fmaxf(__uint_as_float(v[u].z), lo), fmaxf(__uint_as_float(v[u].w), lo), 1);
+      add(fmaxf(__uint_as_float(v[u].x), lo), fmaxf(__uint_as_float(v[u].y), lo));
+      add(fmaxf(__uint_as_float(v[u].z), lo), fmaxf(__uint_as_float(v[u].w), lo));
     }
   } else {
     typedef typename Elem<T>::Two Two;
@@ -244,7 +249,7 @@ __device__ __forceinline__ void add_tile(const uint4 (&v)[kWords], float m, floa
         const unsigned int x = piece(v[u], q);
         const Two h = __hmax2(*reinterpret_cast<const Two*>(&x), lo2);
         const float2 f = Elem<T>::pair(*reinterpret_cast<const unsigned int*>(&h));
-        add(f.x, f.y, q & 1);
+        add(f.x, f.y);
       }
   }
 }
@@ -355,7 +360,7 @@ template <typename T>
 __device__ __forceinline__ bool list_candidates(Shared& sh, const uint4* tile, int words, int first, bool cand,
                                                 float value, int every) {
   constexpr int kPer = Elem<T>::kPerWord;
-  static_assert(kWords * 4 == 32, "a lane's words are one piece per lane");
+  static_assert(kWords * 4 <= 32, "a lane's words are one piece per lane");
   const int lane = threadIdx.x & 31, word = (lane >> 2) * 32;
   const unsigned int* piece_of = reinterpret_cast<const unsigned int*>(tile + word) + (lane & 3);
   bool due = false;
@@ -370,7 +375,7 @@ __device__ __forceinline__ bool list_candidates(Shared& sh, const uint4* tile, i
   if (*static_cast<volatile int*>(&sh.n) > kList) return false;
   for (unsigned int left = __ballot_sync(~0u, cand); left; left &= left - 1) {
     const int from = __ffs(left) - 1;
-    if (from + word < words) {
+    if ((kWords == 8 || lane < 4 * kWords) && from + word < words) {
       const unsigned int x = piece_of[4 * from];
       const int at = first + (from + word) * kPer + (lane & 3) * (kPer / 4);
       if constexpr (kPer == 8) {
@@ -583,19 +588,18 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const P
   const int mine = (tiles - warp + kWarps - 1) / kWarps;  // (0 or less: none)
 
   auto fill = [&](int i) {  // the warp's tile i, by one lane
-    const int st = i % kStages, from = (warp + i * kWarps) * kTileWords;
+    const int from = (warp + i * kWarps) * kTileWords;
     const uint32_t bytes = 16u * min(kTileWords, words - from);
-    sm100::mbar_arrive_expect_tx(&sh.full[warp][st], bytes);
-    bulk_load(sh.ring[warp][st], data + from, bytes, &sh.full[warp][st]);
+    sm100::mbar_arrive_expect_tx(&sh.full[warp], bytes);
+    bulk_load(sh.slot[warp], data + from, bytes, &sh.full[warp]);
   };
   if (lane == 0) {
-    for (int i = 0; i < kStages; ++i) sm100::mbar_init(&sh.full[warp][i], 1);
+    sm100::mbar_init(&sh.full[warp], 1);
     sm100::fence_mbar_init();
-    for (int i = 0; i < min(kStages, mine); ++i) fill(i);
+    if (mine > 0) fill(0);
   }
   if (splits > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
-  // The token now, its logit once a tile has been waited for: neither load is waited for alone.
-  int tok = p.token_ids ? p.token_ids[row] : -1;
+  const int tok = p.token_ids ? p.token_ids[row] : -1;
   float given = __int_as_float(0x7f800000);
   for (int i = tid; i < kList; i += kThreads) sh.list[i] = 0;
   if (tid == 0) {
@@ -608,15 +612,14 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const P
   // holds m (acc_*), of the tiles before it (s, w) and of that tile itself (p_ref), which is kept
   // apart because it is summed again without m in the end.
   float m = neg_inf(), mc = 0.f, s = 0.f, w = 0.f, p_ref = 0.f;
-  u64 acc_s[2] = {0, 0}, acc_w[2] = {0, 0};
+  u64 acc_s = 0, acc_w = 0;
   int ref_tile = -1;  // (-1: the head and tail logits)
-  int above = 0;
-  bool skipped = false;
+  int above = 0;      // (kSkipped: a bit of it)
   auto flush = [&]() {
-    const float2 a = unpack2(add2(acc_s[0], acc_s[1])), b = unpack2(add2(acc_w[0], acc_w[1]));
+    const float2 a = unpack2(acc_s), b = unpack2(acc_w);
     s += a.x + a.y;
     w += b.x + b.y;
-    acc_s[0] = acc_s[1] = acc_w[0] = acc_w[1] = 0;
+    acc_s = acc_w = 0;
   };
   auto raise_to = [&](float top, int tile) {  // s, w and p_ref move to the reference `top`
     const float to = top * kLog2e, dt = bounded(m == neg_inf() ? -1000.f : mc - to), f = fast_exp2(dt);
@@ -628,50 +631,22 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const P
     mc = to;
     ref_tile = tile;
   };
-  float lone = neg_inf();  // a lane's head or tail logit
-  if (part == 0 && warp == 0) {
-    if (lane < head + tail) {
-      const int j = lane < head ? lane : p.vocab - tail + (lane - head);
-      lone = Elem<T>::load(x, j);
-    }
-    __syncwarp();
-    const float top = warp_max_nan(lone != lone ? neg_inf() : lone);
-    if (top >= kLow) {
-      raise_to(top, -1);
-      if (!(lone < kLow)) {
-        const float t = exponent(fmaxf(lone, m - 100.f), mc), e = lone != lone ? lone : fast_exp2(t);
-        p_ref = e;
-        w = e * t;
-      }
-    } else if (top > neg_inf()) {
-      skipped = true;
-    }
-    if (lone != lone) s = lone;
-  }
-
-  bool late = false;
   const int every = k <= 8 ? 8 : k <= 16 ? 16 : 32;
   for (int i = 0; i < max(mine, 1); ++i) {
-    const int st = i % kStages, from = (warp + i * kWarps) * kTileWords;
+    const int from = (warp + i * kWarps) * kTileWords;
     const int nw = words - from;  // words from this tile on
-    if (i < mine && !wait_full(&sh.full[warp][st], (i / kStages) & 1)) late = true;
-    if (i == 0) {
-      if (tok >= 0 && tok < p.vocab) {
-        given = Elem<T>::load(x, tok);
-      } else if (tok != -1) {
-        if (tid == 0 && part == 0 && p.error_bits) atomicOr(p.error_bits, kErrTokenId);
-        tok = -1;
-      }
-    }
+    if (i < mine && !wait_full(&sh.full[warp], i & 1) && p.error_bits) atomicOr(p.error_bits, kErrTimeout);
+    // The given logit once a tile has been waited for: it is not waited for alone.
+    if (i == 0 && tok >= 0 && tok < p.vocab) given = Elem<T>::load(x, tok);
     uint4 v[kWords];
     if (nw >= kTileWords) {
 #pragma unroll
-      for (int u = 0; u < kWords; ++u) v[u] = sh.ring[warp][st][lane + u * 32];
+      for (int u = 0; u < kWords; ++u) v[u] = sh.slot[warp][lane + u * 32];
     } else {
 #pragma unroll
       for (int u = 0; u < kWords; ++u) {
         const int a = lane + u * 32;
-        v[u] = a < nw ? sh.ring[warp][st][a]
+        v[u] = a < nw ? sh.slot[warp][a]
                       : make_uint4(Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest);
       }
     }
@@ -709,15 +684,13 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const P
         }
         if (low && lane == 0) atomicMax(&sh.threshold, ((u64)low << 32) - 1);
         __syncwarp();
-        const u64 key = make_key(lone, lane < head ? lane : p.vocab - tail + (lane - head));
-        if (key > *static_cast<volatile u64*>(&sh.threshold)) sh.list[atomicAdd(&sh.n, 1)] = key;
       }
       const float thr_value = value_of_order(reinterpret_cast<volatile unsigned int*>(&sh.threshold)[1]);
       const bool cand = tm >= thr_value;
-      if (__any_sync(~0u, cand)) due = list_candidates<T>(sh, sh.ring[warp][st], nw, first, cand, thr_value, every);
+      if (__any_sync(~0u, cand)) due = list_candidates<T>(sh, sh.slot[warp], nw, first, cand, thr_value, every);
     }
-    __syncwarp();  // the ring slot is read
-    if (lane == 0 && i + kStages < mine) fill(i + kStages);
+    __syncwarp();  // the slot is read
+    if (lane == 0 && i + 1 < mine) fill(i + 1);
 
     // ---- sums, while the next tiles arrive
     const bool raise = top > m && top >= kLow;
@@ -728,17 +701,39 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const P
     // A tile far below the reference (banned tokens) adds nothing.
     if (top >= m - 120.f) add_tile<T>(v, m, mc, acc_s, acc_w);
     if (top != top) s = top;
-    else if (m == neg_inf() && top > neg_inf()) skipped = true;
+    else if (m == neg_inf() && top > neg_inf()) above |= kSkipped;
     if (raise) {
-      const float2 a = unpack2(add2(acc_s[0], acc_s[1]));
+      const float2 a = unpack2(acc_s);
       p_ref = a.x + a.y;
-      acc_s[0] = acc_s[1] = 0;
+      acc_s = 0;
     }
     if (top > given) above += count_above<T>(v, given);
     if (due) raise_threshold(sh, k);
   }
   flush();
-  above += lone > given;
+  float lone = neg_inf();  // a lane's head or tail logit
+  if (part == 0 && warp == 0 && head + tail > 0) {
+    const int at = lane < head ? lane : p.vocab - tail + (lane - head);
+    if (lane < head + tail) lone = Elem<T>::load(x, at);
+    const float top = warp_max_nan(lone);
+    if (top > m && top >= kLow) raise_to(top, -1);
+    if (lone >= kLow) {
+      const float t = exponent(fmaxf(lone, low_end<T>(m)), mc), e = fast_exp2(t);
+      if (ref_tile < 0) p_ref = e;
+      else s += e;
+      w = fmaf(e, t, w);
+    }
+    if (top != top) s = top;
+    else if (m == neg_inf() && top > neg_inf()) above |= kSkipped;
+    above += lone > given;
+    if (k) {
+      const u64 key = make_key(lone, at);
+      if (key > *static_cast<volatile u64*>(&sh.threshold)) {
+        const int to = atomicAdd(&sh.n, 1);
+        if (to < kList) sh.list[to] = key;
+      }
+    }
+  }
 
   // ---- this CTA's sums about its maximum
   {
@@ -759,12 +754,12 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const P
       int mine = 0;  // logits equal to the maximum
       if (ref_tile < 0) {
         mine = lone == M;
-        if (!mine && !(lone < kLow)) rest += fast_exp2(exponent(fmaxf(lone, m - 100.f), mc));
+        if (!mine && !(lone < kLow)) rest += fast_exp2(exponent(fmaxf(lone, low_end<T>(m)), mc));
       } else {
         const int first = (warp + ref_tile * kWarps) * kTileWords + lane;
         auto take = [&](float f) {
           if (f == M) ++mine;
-          else rest += fast_exp2(exponent(fmaxf(f, m - 100.f), mc));
+          else rest += fast_exp2(exponent(fmaxf(f, low_end<T>(m)), mc));
         };
 #pragma unroll 1
         for (int u = 0; u < kWords; ++u) {
@@ -794,13 +789,13 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const P
     const float all = s + p_ref, q = (w - t0 * (all + (owner == warp && lane == 0 ? fast_exp2(t0) : 0.f))) * inv;
     const float dt = bounded((m - M) * kLog2e), f = fast_exp2(dt);
     const float r_sum = warp_sum(f * inv * all), w_sum = warp_sum(f * fmaf(inv * all, dt, q));
-    const int up = __reduce_add_sync(~0u, above);
+    const unsigned int skipped = __reduce_or_sync(~0u, (unsigned int)above) & (unsigned int)kSkipped;
+    const int up = __reduce_add_sync(~0u, above & INT_MAX);
     if (lane == 0) {
       sh.warp_f[1][warp] = r_sum;
       sh.warp_f[2][warp] = w_sum;
-      sh.warp_above[warp] = up | (skipped ? kSkipped : 0);
+      sh.warp_above[warp] = up | (int)skipped;
     }
-    if (__any_sync(~0u, late) && lane == 0 && p.error_bits) atomicOr(p.error_bits, kErrTimeout);
     __syncthreads();
     if (k) {
       int n = sh.n;
@@ -846,11 +841,13 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const P
   }
 
   // ---- the row
+  const bool has_token = tok >= 0 && tok < p.vocab;
+  if (tid == 0 && !has_token && tok != -1 && p.error_bits) atomicOr(p.error_bits, kErrTokenId);
   Part a = sh.parts[0];
   for (int i = 1; i < splits; ++i) a = join(a, sh.parts[i]);
   if (a.r != a.r || a.w != a.w || a.m > kHighRow ||
       ((a.above & kSkipped) && !(a.m > kLowRow))) {
-    general_row<T>(sh, p, x, row, tok);
+    general_row<T>(sh, p, x, row, has_token ? tok : -1);
     return;
   }
   a.above &= INT_MAX;
@@ -863,8 +860,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const P
   const float nan = __int_as_float(0x7fffffff);
   const float ln_s = a.m == neg_inf() ? nan : log1pf(a.r);
   if (tid == 0) {
-    if (p.logprobs) p.logprobs[row] = tok >= 0 ? (given - a.m) - ln_s : nan;
-    if (p.ranks) p.ranks[row] = tok >= 0 ? 1 + a.above : 0;
+    if (p.logprobs) p.logprobs[row] = has_token ? (given - a.m) - ln_s : nan;
+    if (p.ranks) p.ranks[row] = has_token ? 1 + a.above : 0;
     if (p.entropy) p.entropy[row] = ln_s - kLn2 * (a.w / (1.f + a.r));
   }
   if (tid < k) {
