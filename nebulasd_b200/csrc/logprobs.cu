@@ -36,7 +36,7 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kWords = 8;                  // 16-byte words per lane and tile
 constexpr int kTileWords = 32 * kWords;    // of one warp: 4 KB
-constexpr int kCtas = 4;                   // resident per SM
+constexpr int kCtas = 3;                   // resident per SM
 constexpr int kMaxTop = NEB_MAX_TOP_LOGPROBS;
 constexpr int kMaxSplits = 8;              // CTAs per row (the portable cluster size)
 constexpr int kList = 512;                 // candidates
@@ -51,7 +51,7 @@ typedef unsigned long long u64;
 struct Params {
   const void* logits;
   long long row_stride;
-  int vocab, num_rows, num_top, splits;
+  int vocab, num_rows, num_top, splits, log_splits;  // splits = 1 << log_splits CTAs per row
   const int32_t* token_ids;
   float* logprobs;
   int32_t* ranks;
@@ -71,11 +71,12 @@ constexpr int kSkipped = INT_MIN;  // a tile below kLow was left out
 struct Shared {
   uint4 slot[kWarps][kTileWords];
   u64 list[kList];
-  u64 sorted[kMaxTop];
+  u64 sorted[kMaxTop], merged[kMaxTop];  // the part's largest keys, the row's
   Part parts[kMaxSplits];
-  u64 gathered[kMaxSplits][kMaxTop];
+  u64 gathered[kMaxSplits * kMaxTop];  // num_top of each part
   uint64_t full[kWarps];
   u64 warp_key[kWarps];
+  int first_index[kWarps];  // of each warp's range
   unsigned int tops[64];
   u64 threshold;  // only larger keys are listed; num_top listed ones are at or above it
   float warp_f[3][kWarps];
@@ -155,12 +156,12 @@ __device__ __forceinline__ unsigned int piece(const uint4& v, int q) {
   return q == 0 ? v.x : q == 1 ? v.y : q == 2 ? v.z : v.w;
 }
 // NaN if there is one.
-template <typename T>
-__device__ __forceinline__ float words_max(const uint4 (&v)[kWords]) {
+template <typename T, int N>
+__device__ __forceinline__ float words_max(const uint4 (&v)[N]) {
   if constexpr (Elem<T>::kPerWord == 4) {
     float m = neg_inf();
 #pragma unroll
-    for (int u = 0; u < kWords; ++u)
+    for (int u = 0; u < N; ++u)
 #pragma unroll
       for (int q = 0; q < 4; ++q) m = max_nan(m, __uint_as_float(piece(v[u], q)));
     return m;
@@ -169,7 +170,7 @@ __device__ __forceinline__ float words_max(const uint4 (&v)[kWords]) {
     const unsigned int low = Elem<T>::kLowest;
     Two m = *reinterpret_cast<const Two*>(&low);
 #pragma unroll
-    for (int u = 0; u < kWords; ++u)
+    for (int u = 0; u < N; ++u)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const unsigned int x = piece(v[u], q);
@@ -214,16 +215,27 @@ __device__ __forceinline__ float warp_max_nan(float v) {
 // itself is t0, not 0; e0 = 2^t0 takes that out of the finished sums.
 __device__ __forceinline__ float exponent(float x, float mc) { return fmaf(x, kLog2e, -mc); }
 
+// Moves the sums to the reference `top`.
+__device__ __forceinline__ void move_up(float top, float& m, float& mc, float& s, float& w, float& p_ref) {
+  const float to = top * kLog2e, dt = bounded(m == neg_inf() ? -1000.f : mc - to), f = fast_exp2(dt);
+  const float all = s + p_ref;
+  w = f * fmaf(all, dt, w);
+  s = f * all;
+  p_ref = 0.f;
+  m = top;
+  mc = to;
+}
+
 // Where logits far below the reference are cut off: their terms are 0 all the same.
 template <typename T>
 __device__ __forceinline__ float low_end(float m) {
   return fmaxf(m - 100.f - fabsf(m) * Elem<T>::kUlp, kFinite);
 }
 
-// Adds a tile's terms 2^t and 2^t t, two fp32 lanes per instruction.  The cut-off keeps
+// Adds the words' terms 2^t and 2^t t, two fp32 lanes per instruction.  The cut-off keeps
 // 0 times -inf out of the second sum.
-template <typename T>
-__device__ __forceinline__ void add_tile(const uint4 (&v)[kWords], float m, float mc, u64& s, u64& w) {
+template <typename T, int N>
+__device__ __forceinline__ void add_words(const uint4 (&v)[N], float m, float mc, u64& s, u64& w) {
   const u64 c2 = pack2(kLog2e, kLog2e), mc2 = pack2(-mc, -mc);
   const float lo = low_end<T>(m);
   auto add = [&](float a, float b) {
@@ -235,7 +247,7 @@ __device__ __forceinline__ void add_tile(const uint4 (&v)[kWords], float m, floa
   };
   if constexpr (Elem<T>::kPerWord == 4) {
 #pragma unroll
-    for (int u = 0; u < kWords; ++u) {
+    for (int u = 0; u < N; ++u) {
       add(fmaxf(__uint_as_float(v[u].x), lo), fmaxf(__uint_as_float(v[u].y), lo));
       add(fmaxf(__uint_as_float(v[u].z), lo), fmaxf(__uint_as_float(v[u].w), lo));
     }
@@ -243,7 +255,7 @@ __device__ __forceinline__ void add_tile(const uint4 (&v)[kWords], float m, floa
     typedef typename Elem<T>::Two Two;
     const Two lo2 = Elem<T>::twice(lo);
 #pragma unroll
-    for (int u = 0; u < kWords; ++u)
+    for (int u = 0; u < N; ++u)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const unsigned int x = piece(v[u], q);
@@ -254,13 +266,13 @@ __device__ __forceinline__ void add_tile(const uint4 (&v)[kWords], float m, floa
   }
 }
 
-// Logits of a tile larger than `given`.
-template <typename T>
-__device__ __forceinline__ int count_above(const uint4 (&v)[kWords], float given) {
+// Logits larger than `given`.
+template <typename T, int N>
+__device__ __forceinline__ int count_above(const uint4 (&v)[N], float given) {
   if constexpr (Elem<T>::kPerWord == 4) {
     int n = 0;
 #pragma unroll
-    for (int u = 0; u < kWords; ++u)
+    for (int u = 0; u < N; ++u)
 #pragma unroll
       for (int q = 0; q < 4; ++q) n += __uint_as_float(piece(v[u], q)) > given;
     return n;
@@ -270,7 +282,7 @@ __device__ __forceinline__ int count_above(const uint4 (&v)[kWords], float given
     // Masks 0xffff add up to 65536 (low - high) - low in 32 bits.
     unsigned int sum = 0;
 #pragma unroll
-    for (int u = 0; u < kWords; ++u)
+    for (int u = 0; u < N; ++u)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const unsigned int x = piece(v[u], q);
@@ -341,28 +353,30 @@ __device__ __forceinline__ u64 search(Shared& sh, int& turn, u64 lo, int lowest,
   return lo;
 }
 
-// The list's num_top largest keys in order (0 where there are fewer) into sh.sorted, by counting.
-__device__ __forceinline__ void rank_list(Shared& sh, int n, int num_top) {
-  for (int i = threadIdx.x + n; i < num_top; i += kThreads) sh.sorted[i] = 0;
+// The num_top largest of n keys in order into `sorted`, by counting; its places beyond n keep their 0.  Keys of
+// 0 are none.
+__device__ __forceinline__ void rank_keys(const u64* keys, int n, int num_top, u64* sorted) {
   for (int i = threadIdx.x; i < n; i += kThreads) {
-    const u64 key = sh.list[i];
+    const u64 key = keys[i];
     int before = 0;
-    for (int j = 0; j < n; ++j) before += sh.list[j] > key;
-    if (before < num_top) sh.sorted[before] = key;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) before += keys[j] > key;
+    if (key && before < num_top) sorted[before] = key;
   }
   __syncthreads();
 }
 
 // Lists the logits above the threshold among the words of the warp's candidate lanes, a 32-bit piece of the
-// tile per lane.  `first`: the index of the tile's first logit, `value` the threshold's.  True when it is time for
-// a better threshold: after every `every`-th candidate (a power of two).
+// tile per lane.  `from`: the tile's first word in the warp's range, `value` the threshold's.  True when it is time
+// for a better threshold.
 template <typename T>
-__device__ __forceinline__ bool list_candidates(Shared& sh, const uint4* tile, int words, int first, bool cand,
-                                                float value, int every) {
+__device__ __forceinline__ bool list_candidates(Shared& sh, int from, int words, bool cand, float value, int k) {
   constexpr int kPer = Elem<T>::kPerWord;
-  static_assert(kWords * 4 <= 32, "a lane's words are one piece per lane");
-  const int lane = threadIdx.x & 31, word = (lane >> 2) * 32;
-  const unsigned int* piece_of = reinterpret_cast<const unsigned int*>(tile + word) + (lane & 3);
+  static_assert(kWords * 4 == 32, "a lane's words are one piece per lane");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, word = (lane >> 2) * 32;
+  const unsigned int* piece_of = reinterpret_cast<const unsigned int*>(sh.slot[warp] + word) + (lane & 3);
+  const int first = sh.first_index[warp] + from * kPer;
+  const int every = k <= 8 ? 8 : k <= 16 ? 16 : 32;
   bool due = false;
   auto offer = [&](float f, int idx) {
     const u64 key = make_key(f, idx);
@@ -374,10 +388,10 @@ __device__ __forceinline__ bool list_candidates(Shared& sh, const uint4* tile, i
   };
   if (*static_cast<volatile int*>(&sh.n) > kList) return false;
   for (unsigned int left = __ballot_sync(~0u, cand); left; left &= left - 1) {
-    const int from = __ffs(left) - 1;
-    if ((kWords == 8 || lane < 4 * kWords) && from + word < words) {
-      const unsigned int x = piece_of[4 * from];
-      const int at = first + (from + word) * kPer + (lane & 3) * (kPer / 4);
+    const int other = __ffs(left) - 1;
+    if (other + word < words) {
+      const unsigned int x = piece_of[4 * other];
+      const int at = first + (other + word) * kPer + (lane & 3) * (kPer / 4);
       if constexpr (kPer == 8) {
         const float2 f = Elem<T>::pair(x);
         if (f.x >= value) offer(f.x, at);
@@ -436,7 +450,9 @@ __device__ __noinline__ int collect(Shared& sh, const uint4* data, int words, in
       if (key[j] > thr) sh.list[atomicAdd(&sh.n, 1)] = key[j];
     __syncthreads();
     n = sh.n;
-    rank_list(sh, n, k);
+    if (tid < k) sh.sorted[tid] = 0;
+    __syncthreads();
+    rank_keys(sh.list, n, k, sh.sorted);
     n = min(n, k);
     if (tid < n) sh.list[tid] = sh.sorted[tid];
     if (n == k) thr = sh.sorted[k - 1] > thr ? sh.sorted[k - 1] : thr;
@@ -445,10 +461,10 @@ __device__ __noinline__ int collect(Shared& sh, const uint4* data, int words, in
   return n;
 }
 
-// Fills sh.sorted from n to k with the logits below kLow, which the candidates leave out: largest first (all of
+// Fills `sorted` from n to k with the logits below kLow, which the candidates leave out: largest first (all of
 // them mostly equal, -inf or another mask), then by index.
 template <typename T>
-__device__ __noinline__ void fill_masked(Shared& sh, const void* x, int vocab, int n, int k) {
+__device__ __noinline__ void fill_masked(Shared& sh, u64* sorted, const void* x, int vocab, int n, int k) {
   const int tid = threadIdx.x;
   int turn = 0;
   float limit = kLow;
@@ -476,12 +492,48 @@ __device__ __noinline__ void fill_masked(Shared& sh, const void* x, int vocab, i
         all += sh.warp_count[turn][i];
       }
       turn ^= 1;
-      if (hit && n + before < k) sh.sorted[n + before] = ((u64)best << 32) | (unsigned int)~(unsigned int)j;
+      if (hit && n + before < k) sorted[n + before] = ((u64)best << 32) | (unsigned int)~(unsigned int)j;
       n += all;
     }
     limit = value_of_order(best);
   }
   __syncthreads();
+}
+
+// A lane's terms of the tile at `data`, but for the logits equal to the maximum M, which it counts.  (All loads
+// come before the first use, so that the warp waits once.)
+template <typename T>
+__device__ __noinline__ float tile_without(const uint4* data, int words, float M, float m, float mc, int& equal) {
+  uint4 v[kWords];
+#pragma unroll
+  for (int u = 0; u < kWords; ++u) {
+    const int a = (threadIdx.x & 31) + u * 32;
+    v[u] = a < words ? __ldg(data + a)
+                     : make_uint4(Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest);
+  }
+  const float lo = low_end<T>(m);
+  float sum = 0.f;
+  int n = 0;
+  auto take = [&](float f) {
+    const float e = fast_exp2(exponent(fmaxf(f, lo), mc));
+    n += f == M;
+    sum += f == M ? 0.f : e;
+  };
+#pragma unroll
+  for (int u = 0; u < kWords; ++u) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if constexpr (Elem<T>::kPerWord == 8) {
+        const float2 f = Elem<T>::pair(piece(v[u], q));
+        take(f.x);
+        take(f.y);
+      } else {
+        take(__uint_as_float(piece(v[u], q)));
+      }
+    }
+  }
+  equal = n;
+  return sum;
 }
 
 // Joins `b` into `a`: sums about the larger maximum, which alone is left out of r.
@@ -567,156 +619,48 @@ __device__ __noinline__ void general_row(Shared& sh, const Params& p, const void
   }
 }
 
-// --------------------------------------------------------------------- kernel
+// What the CTA reads: [head logits][16-byte words][tail logits] of its row, the words in parts, a part in a range
+// for each warp.
 template <typename T>
-__global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const Params p) {
-  extern __shared__ __align__(128) unsigned char smem_raw[];
-  Shared& sh = *reinterpret_cast<Shared*>(smem_raw);
-  constexpr int kPer = Elem<T>::kPerWord;
+struct Place {
+  const T* x;
+  const uint4* data;  // the part's words
+  int row, part, head, tail, w0, words, share;  // of the row; of the part; words of a warp
+  __device__ __forceinline__ explicit Place(const Params& p) {
+    row = blockIdx.x >> p.log_splits;
+    part = blockIdx.x & (p.splits - 1);
+    x = static_cast<const T*>(p.logits) + (long long)row * p.row_stride;
+    head = min(p.vocab, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
+    const int all = (p.vocab - head) / Elem<T>::kPerWord;
+    tail = p.vocab - head - all * Elem<T>::kPerWord;
+    w0 = (int)(((long long)all * part) >> p.log_splits);
+    words = (int)(((long long)all * (part + 1)) >> p.log_splits) - w0;
+    data = reinterpret_cast<const uint4*>(x + head) + w0;
+    share = ((words + kThreads - 1) / kThreads) * 32;
+  }
+  __device__ __forceinline__ int first_word() const { return (int)(threadIdx.x >> 5) * share; }
+  __device__ __forceinline__ int mine() const { return min(share, words - first_word()); }  // (0 or less: none)
+  __device__ __forceinline__ int index(int word) const { return head + (w0 + word) * Elem<T>::kPerWord; }
+};
+
+// --------------------------------------------------------------------- kernel
+// The rest of a row part: head and tail logits, the sums of the warps and of the parts, the row's results.  Out of
+// line, so that its registers are not the loop's.
+template <typename T>
+__device__ __noinline__ void finish(Shared& sh, const Params& p, float m, float mc, float s, float w, float p_ref,
+                                    float given, int above, int ref_tile) {
+  const Place<T> at(p);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int splits = p.splits, row = blockIdx.x / splits, part = blockIdx.x - row * splits;
-  const T* x = static_cast<const T*>(p.logits) + (long long)row * p.row_stride;
-  const int k = p.num_top;
-
-  // [head logits][16-byte words][tail logits]; the CTA's words go round its warps in tiles.
-  const int head = min(p.vocab, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
-  const int row_words = (p.vocab - head) / kPer, tail = p.vocab - head - row_words * kPer;
-  const int w0 = (int)((long long)row_words * part / splits);
-  const int words = (int)((long long)row_words * (part + 1) / splits) - w0;
-  const uint4* data = reinterpret_cast<const uint4*>(x + head) + w0;
-  const int tiles = (words + kTileWords - 1) / kTileWords;
-  const int mine = (tiles - warp + kWarps - 1) / kWarps;  // (0 or less: none)
-
-  auto fill = [&](int i) {  // the warp's tile i, by one lane
-    const int from = (warp + i * kWarps) * kTileWords;
-    const uint32_t bytes = 16u * min(kTileWords, words - from);
-    sm100::mbar_arrive_expect_tx(&sh.full[warp], bytes);
-    bulk_load(sh.slot[warp], data + from, bytes, &sh.full[warp]);
-  };
-  if (lane == 0) {
-    sm100::mbar_init(&sh.full[warp], 1);
-    sm100::fence_mbar_init();
-    if (mine > 0) fill(0);
-  }
-  if (splits > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
-  const int tok = p.token_ids ? p.token_ids[row] : -1;
-  float given = __int_as_float(0x7f800000);
-  for (int i = tid; i < kList; i += kThreads) sh.list[i] = 0;
-  if (tid == 0) {
-    sh.n = 0;
-    sh.threshold = ((u64)order_f32(kLow) << 32) - 1;  // masked logits are no candidates
-  }
-  __syncwarp();
-
-  // Per warp: the reference m, rounded to mc in base 2.  Per lane: sums of the tiles since the one that
-  // holds m (acc_*), of the tiles before it (s, w) and of that tile itself (p_ref), which is kept
-  // apart because it is summed again without m in the end.
-  float m = neg_inf(), mc = 0.f, s = 0.f, w = 0.f, p_ref = 0.f;
-  u64 acc_s = 0, acc_w = 0;
-  int ref_tile = -1;  // (-1: the head and tail logits)
-  int above = 0;      // (kSkipped: a bit of it)
-  auto flush = [&]() {
-    const float2 a = unpack2(acc_s), b = unpack2(acc_w);
-    s += a.x + a.y;
-    w += b.x + b.y;
-    acc_s = acc_w = 0;
-  };
-  auto raise_to = [&](float top, int tile) {  // s, w and p_ref move to the reference `top`
-    const float to = top * kLog2e, dt = bounded(m == neg_inf() ? -1000.f : mc - to), f = fast_exp2(dt);
-    const float all = s + p_ref;
-    w = f * fmaf(all, dt, w);
-    s = f * all;
-    p_ref = 0.f;
-    m = top;
-    mc = to;
-    ref_tile = tile;
-  };
-  const int every = k <= 8 ? 8 : k <= 16 ? 16 : 32;
-  for (int i = 0; i < max(mine, 1); ++i) {
-    const int from = (warp + i * kWarps) * kTileWords;
-    const int nw = words - from;  // words from this tile on
-    if (i < mine && !wait_full(&sh.full[warp], i & 1) && p.error_bits) atomicOr(p.error_bits, kErrTimeout);
-    // The given logit once a tile has been waited for: it is not waited for alone.
-    if (i == 0 && tok >= 0 && tok < p.vocab) given = Elem<T>::load(x, tok);
-    uint4 v[kWords];
-    if (nw >= kTileWords) {
-#pragma unroll
-      for (int u = 0; u < kWords; ++u) v[u] = sh.slot[warp][lane + u * 32];
-    } else {
-#pragma unroll
-      for (int u = 0; u < kWords; ++u) {
-        const int a = lane + u * 32;
-        v[u] = a < nw ? sh.slot[warp][a]
-                      : make_uint4(Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest);
-      }
-    }
-    const float tm = words_max<T>(v), top = warp_max_nan(tm);
-
-    // ---- candidates
-    bool due = false;
-    if (k) {
-      const int first = head + (w0 + from) * kPer;  // index of the tile's first logit
-      if (i == 0) {
-        // The first threshold: the k-th largest of the top lane maxima of each warp whose lanes all have logits.
-        const int whole = words >= 32 ? min(kWarps, (words - 32) / kTileWords + 1) : 0;
-        const int each = whole == kWarps ? min(k, 4) : whole ? (k + whole - 1) / whole : 0;
-        unsigned int o = tm >= kLow ? order_f32(tm) : 0u;
-        if (warp < whole) {
-          for (int j = 0; j < each; ++j) {
-            const unsigned int best = __reduce_max_sync(~0u, o);
-            const unsigned int who = __ballot_sync(~0u, o == best);
-            if (lane == __ffs(who) - 1) {
-              sh.tops[warp * each + j] = best;
-              o = 0;
-            }
-          }
-        }
-        __syncthreads();
-        unsigned int a = lane < whole * each ? sh.tops[lane] : 0u, b = lane + 32 < whole * each ? sh.tops[lane + 32] : 0u;
-        unsigned int low = 0;
-        for (int j = 0; j < k && whole; ++j) {
-          low = __reduce_max_sync(~0u, max(a, b));
-          const unsigned int who = __ballot_sync(~0u, max(a, b) == low);
-          if (lane == __ffs(who) - 1) {
-            if (a == low) a = 0;
-            else b = 0;
-          }
-        }
-        if (low && lane == 0) atomicMax(&sh.threshold, ((u64)low << 32) - 1);
-        __syncwarp();
-      }
-      const float thr_value = value_of_order(reinterpret_cast<volatile unsigned int*>(&sh.threshold)[1]);
-      const bool cand = tm >= thr_value;
-      if (__any_sync(~0u, cand)) due = list_candidates<T>(sh, sh.slot[warp], nw, first, cand, thr_value, every);
-    }
-    __syncwarp();  // the slot is read
-    if (lane == 0 && i + 1 < mine) fill(i + 1);
-
-    // ---- sums, while the next tiles arrive
-    const bool raise = top > m && top >= kLow;
-    if (raise) {
-      flush();
-      raise_to(top, i);
-    }
-    // A tile far below the reference (banned tokens) adds nothing.
-    if (top >= m - 120.f) add_tile<T>(v, m, mc, acc_s, acc_w);
-    if (top != top) s = top;
-    else if (m == neg_inf() && top > neg_inf()) above |= kSkipped;
-    if (raise) {
-      const float2 a = unpack2(acc_s);
-      p_ref = a.x + a.y;
-      acc_s = 0;
-    }
-    if (top > given) above += count_above<T>(v, given);
-    if (due) raise_threshold(sh, k);
-  }
-  flush();
+  const int splits = p.splits, row = at.row, part = at.part, head = at.head, tail = at.tail, k = p.num_top;
   float lone = neg_inf();  // a lane's head or tail logit
   if (part == 0 && warp == 0 && head + tail > 0) {
-    const int at = lane < head ? lane : p.vocab - tail + (lane - head);
-    if (lane < head + tail) lone = Elem<T>::load(x, at);
+    const int index = lane < head ? lane : p.vocab - tail + (lane - head);
+    if (lane < head + tail) lone = Elem<T>::load(at.x, index);
     const float top = warp_max_nan(lone);
-    if (top > m && top >= kLow) raise_to(top, -1);
+    if (top > m && top >= kLow) {
+      move_up(top, m, mc, s, w, p_ref);
+      ref_tile = -1;
+    }
     if (lone >= kLow) {
       const float t = exponent(fmaxf(lone, low_end<T>(m)), mc), e = fast_exp2(t);
       if (ref_tile < 0) p_ref = e;
@@ -727,7 +671,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const P
     else if (m == neg_inf() && top > neg_inf()) above |= kSkipped;
     above += lone > given;
     if (k) {
-      const u64 key = make_key(lone, at);
+      const u64 key = make_key(lone, index);
       if (key > *static_cast<volatile u64*>(&sh.threshold)) {
         const int to = atomicAdd(&sh.n, 1);
         if (to < kList) sh.list[to] = key;
@@ -751,37 +695,17 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const P
       // Sum the tile that holds the maximum again, without it.
       const float keep = p_ref != p_ref ? p_ref : 0.f;
       float rest = keep;
-      int mine = 0;  // logits equal to the maximum
+      int equal = 0;  // logits equal to the maximum
       if (ref_tile < 0) {
-        mine = lone == M;
-        if (!mine && !(lone < kLow)) rest += fast_exp2(exponent(fmaxf(lone, low_end<T>(m)), mc));
+        equal = lone == M;
+        if (!equal && !(lone < kLow)) rest += fast_exp2(exponent(fmaxf(lone, low_end<T>(m)), mc));
       } else {
-        const int first = (warp + ref_tile * kWarps) * kTileWords + lane;
-        auto take = [&](float f) {
-          if (f == M) ++mine;
-          else rest += fast_exp2(exponent(fmaxf(f, low_end<T>(m)), mc));
-        };
-#pragma unroll 1
-        for (int u = 0; u < kWords; ++u) {
-          if (first + u * 32 < words) {
-            const uint4 word = __ldg(data + first + u * 32);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              if constexpr (kPer == 8) {
-                const float2 f = Elem<T>::pair(piece(word, q));
-                take(f.x);
-                take(f.y);
-              } else {
-                take(__uint_as_float(piece(word, q)));
-              }
-            }
-          }
-        }
+        rest += tile_without<T>(at.data + at.first_word() + ref_tile, at.mine() - ref_tile, M, m, mc, equal);
       }
-      const unsigned int who = __ballot_sync(~0u, mine > 0);
+      const unsigned int who = __ballot_sync(~0u, equal > 0);
       const float e0 = fast_exp2(exponent(m, mc));
-      if (lane == __ffs(who) - 1) --mine;
-      p_ref = fmaf((float)mine, e0, rest);
+      if (lane == __ffs(who) - 1) --equal;
+      p_ref = fmaf((float)equal, e0, rest);
     }
     // From the rounded reference to m, then to the CTA's maximum.  The maximum itself, left out of the owner's
     // sum, has a term in w: e0 t0.
@@ -799,63 +723,56 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const P
     __syncthreads();
     if (k) {
       int n = sh.n;
-      if (n > kList) n = collect<T>(sh, data, words, head + w0 * kPer, x, p.vocab, part ? 0 : head, part ? 0 : tail, k);
-      rank_list(sh, n, k);
+      if (n > kList) n = collect<T>(sh, at.data, at.words, at.index(0), at.x, p.vocab, part ? 0 : head, part ? 0 : tail, k);
+      rank_keys(sh.list, n, k, sh.sorted);
     }
-    Part mine{M, 0.f, 0.f, 0};
+    Part own{M, 0.f, 0.f, 0};
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) {
-      mine.r += sh.warp_f[1][i];
-      mine.w += sh.warp_f[2][i];
-      mine.above = ((mine.above + sh.warp_above[i]) & INT_MAX) | ((mine.above | sh.warp_above[i]) & kSkipped);
+      own.r += sh.warp_f[1][i];
+      own.w += sh.warp_f[2][i];
+      own.above = ((own.above + sh.warp_above[i]) & INT_MAX) | ((own.above | sh.warp_above[i]) & kSkipped);
     }
     if (splits == 1) {
-      if (tid == 0) sh.parts[0] = mine;
+      if (tid == 0) sh.parts[0] = own;
     } else {
       // Into the first CTA's shared memory.
       asm volatile("barrier.cluster.wait;" ::: "memory");  // it has started
-      uint32_t at;
-      asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(sm100::smem_u32(&sh.parts[part])));
+      uint32_t to;
+      asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(sm100::smem_u32(&sh.parts[part])));
       if (tid == 0)
-        asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(__float_as_uint(mine.m)),
-                     "r"(__float_as_uint(mine.r)), "r"(__float_as_uint(mine.w)), "r"(mine.above)
+        asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(__float_as_uint(own.m)),
+                     "r"(__float_as_uint(own.r)), "r"(__float_as_uint(own.w)), "r"(own.above)
                      : "memory");
-      asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(sm100::smem_u32(&sh.gathered[part][0])));
+      asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(sm100::smem_u32(&sh.gathered[part * k])));
       if (tid < k)
-        asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(at + 8 * tid), "l"(sh.sorted[tid]) : "memory");
+        asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(to + 8 * tid), "l"(sh.sorted[tid]) : "memory");
       asm volatile("barrier.cluster.arrive.release;" ::: "memory");
       if (part != 0) return;
       asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-      if (k) {
-        if (tid == 0) sh.n = 0;
-        __syncthreads();
-        for (int i = tid; i < splits * k; i += kThreads) {
-          const u64 key = sh.gathered[i / k][i % k];
-          if (key) sh.list[atomicAdd(&sh.n, 1)] = key;
-        }
-        __syncthreads();
-        rank_list(sh, sh.n, k);
-      }
+      if (k) rank_keys(sh.gathered, splits * k, k, sh.merged);
     }
     __syncthreads();
   }
 
   // ---- the row
+  const int tok = p.token_ids ? p.token_ids[row] : -1;
   const bool has_token = tok >= 0 && tok < p.vocab;
   if (tid == 0 && !has_token && tok != -1 && p.error_bits) atomicOr(p.error_bits, kErrTokenId);
   Part a = sh.parts[0];
   for (int i = 1; i < splits; ++i) a = join(a, sh.parts[i]);
   if (a.r != a.r || a.w != a.w || a.m > kHighRow ||
       ((a.above & kSkipped) && !(a.m > kLowRow))) {
-    general_row<T>(sh, p, x, row, has_token ? tok : -1);
+    general_row<T>(sh, p, at.x, row, has_token ? tok : -1);
     return;
   }
   a.above &= INT_MAX;
-  if (k && sh.sorted[k - 1] == 0) {
+  u64* top_keys = splits > 1 ? sh.merged : sh.sorted;
+  if (k && top_keys[k - 1] == 0) {
     int listed = 0;
-    while (sh.sorted[listed]) ++listed;
+    while (top_keys[listed]) ++listed;
     __syncthreads();
-    fill_masked<T>(sh, x, p.vocab, listed, k);
+    fill_masked<T>(sh, top_keys, at.x, p.vocab, listed, k);
   }
   const float nan = __int_as_float(0x7fffffff);
   const float ln_s = a.m == neg_inf() ? nan : log1pf(a.r);
@@ -865,19 +782,187 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const P
     if (p.entropy) p.entropy[row] = ln_s - kLn2 * (a.w / (1.f + a.r));
   }
   if (tid < k) {
-    const u64 key = sh.sorted[tid];
+    const u64 key = top_keys[tid];
     p.top_ids[(long long)row * k + tid] = key_index(key);
     p.top_logprobs[(long long)row * k + tid] = (key_value(key) - a.m) - ln_s;
   }
 }
 
+template <typename T>
+__global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const __grid_constant__ Params p) {
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  Shared& sh = *reinterpret_cast<Shared*>(smem_raw);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Place<T> at(p);
+  const uint4* data = at.data + at.first_word();
+  const int mine = at.mine(), k = p.num_top;
+
+  auto fill = [&](int from) {  // the warp's tile from word `from` on, by one lane
+    const uint32_t bytes = 16u * min(kTileWords, mine - from);
+    sm100::mbar_arrive_expect_tx(&sh.full[warp], bytes);
+    bulk_load(sh.slot[warp], data + from, bytes, &sh.full[warp]);
+  };
+  if (lane == 0) {
+    sm100::mbar_init(&sh.full[warp], 1);
+    sm100::fence_mbar_init();
+    if (mine > 0) fill(0);
+  }
+  if (p.splits > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+  const int tok = p.token_ids ? p.token_ids[at.row] : -1;
+  float given = __int_as_float(0x7f800000);
+  for (int i = tid; i < kList; i += kThreads) sh.list[i] = 0;
+  if (tid < kMaxTop) sh.sorted[tid] = sh.merged[tid] = 0;
+  if (tid == 0) {
+    sh.n = 0;
+    sh.threshold = ((u64)order_f32(kLow) << 32) - 1;  // masked logits are no candidates
+  }
+  __syncwarp();
+
+  // Per warp: the reference m, rounded to mc in base 2.  Per lane: sums of the tiles since the one that
+  // holds m (acc_*), of the tiles before it (s, w) and of that tile itself (p_ref), which is kept
+  // apart because it is summed again without m in the end.
+  float m = neg_inf(), mc = 0.f, s = 0.f, w = 0.f, p_ref = 0.f;
+  u64 acc_s = 0, acc_w = 0;
+  int ref_tile = -1;  // its first word (-1: the head and tail logits)
+  int above = 0;      // (kSkipped: a bit of it)
+  auto flush = [&]() {
+    const float2 a = unpack2(acc_s), b = unpack2(acc_w);
+    s += a.x + a.y;
+    w += b.x + b.y;
+    acc_s = acc_w = 0;
+  };
+  if (lane == 0) sh.first_index[warp] = at.index(at.first_word());
+  __syncwarp();
+  for (int from = 0; from == 0 || from < mine; from += kTileWords) {
+    const int nw = mine - from;  // words from this tile on
+    if (nw > 0 && !wait_full(&sh.full[warp], (from / kTileWords) & 1) && p.error_bits)
+      atomicOr(p.error_bits, kErrTimeout);
+    // The given logit once a tile has been waited for: it is not waited for alone.
+    if (from == 0 && tok >= 0 && tok < p.vocab) given = Elem<T>::load(at.x, tok);
+    // A whole tile lies in registers; of the last one, words are read as they are needed.
+    const uint4* slot = sh.slot[warp];
+    const bool whole = nw >= kTileWords;
+    uint4 v[kWords];
+    auto word = [&](int u, uint4 (&one)[1]) {
+      const int a = lane + u * 32;
+      one[0] = a < nw ? slot[a] : make_uint4(Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest);
+    };
+    float tm = neg_inf();
+    if (whole) {
+#pragma unroll
+      for (int u = 0; u < kWords; ++u) v[u] = slot[lane + u * 32];
+      tm = words_max<T>(v);
+    } else {
+      for (int u = 0; u * 32 < nw; ++u) {
+        uint4 one[1];
+        word(u, one);
+        tm = max_nan(tm, words_max<T>(one));
+      }
+    }
+    const float top = warp_max_nan(tm);
+
+    // ---- candidates
+    bool due = false;
+    if (k) {
+      if (from == 0) {
+        // The first threshold: the k-th largest of the top lane maxima of each warp whose lanes all have logits.
+        const int full = at.words >= 32 ? min(kWarps, (at.words - 32) / at.share + 1) : 0;
+        const int each = full == kWarps ? min(k, 4) : full ? (k + full - 1) / full : 0, all = full * each;
+        unsigned int o = tm >= kLow ? order_f32(tm) : 0u;
+        if (warp < full) {
+          for (int j = 0; j < each; ++j) {
+            const unsigned int best = __reduce_max_sync(~0u, o);
+            const unsigned int who = __ballot_sync(~0u, o == best);
+            if (lane == __ffs(who) - 1) {
+              sh.tops[warp * each + j] = best;
+              o = 0;
+            }
+          }
+        }
+        __syncthreads();
+        // Few rounds of maxima, or each place counted: k = 8 costs the same either way.
+        unsigned int low = 0;
+        if (k <= 8) {
+          unsigned int o2 = lane < all ? sh.tops[lane] : 0u;
+          for (int j = 0; j < k && all; ++j) {
+            low = __reduce_max_sync(~0u, o2);
+            const unsigned int who = __ballot_sync(~0u, o2 == low);
+            if (lane == __ffs(who) - 1) o2 = 0;
+          }
+        } else {
+          for (int j = lane; j < all; j += 32) {
+            const unsigned int own_top = sh.tops[j];
+            int larger = 0, least = 0;
+#pragma unroll 4
+            for (int q = 0; q < all; ++q) {
+              larger += sh.tops[q] > own_top;
+              least += sh.tops[q] >= own_top;
+            }
+            if (larger < k && k <= least) low = own_top;
+          }
+          low = __reduce_max_sync(~0u, low);
+        }
+        if (low && lane == 0) atomicMax(&sh.threshold, ((u64)low << 32) - 1);
+        __syncwarp();
+      }
+      const float thr_value = value_of_order(reinterpret_cast<volatile unsigned int*>(&sh.threshold)[1]);
+      const bool cand = tm >= thr_value;
+      if (__any_sync(~0u, cand)) due = list_candidates<T>(sh, from, nw, cand, thr_value, k);
+    }
+    __syncwarp();  // the slot is read
+    if (lane == 0 && from + kTileWords < mine) fill(from + kTileWords);
+
+    // ---- sums, while the next tiles arrive
+    const bool raise = top > m && top >= kLow;
+    if (raise) {
+      flush();
+      move_up(top, m, mc, s, w, p_ref);
+      ref_tile = from;
+    }
+    // A tile far below the reference (banned tokens) adds nothing.
+    if (top >= m - 120.f) {
+      if (whole) {
+        add_words<T>(v, m, mc, acc_s, acc_w);
+      } else {
+        for (int u = 0; u * 32 < nw; ++u) {
+          uint4 one[1];
+          word(u, one);
+          add_words<T>(one, m, mc, acc_s, acc_w);
+        }
+      }
+    }
+    if (top != top) s = top;
+    else if (m == neg_inf() && top > neg_inf()) above |= kSkipped;
+    if (raise) {
+      const float2 a = unpack2(acc_s);
+      p_ref = a.x + a.y;
+      acc_s = 0;
+    }
+    if (top > given) {
+      if (whole) {
+        above += count_above<T>(v, given);
+      } else {
+        for (int u = 0; u * 32 < nw; ++u) {
+          uint4 one[1];
+          word(u, one);
+          above += count_above<T>(one, given);
+        }
+      }
+    }
+    if (due) raise_threshold(sh, k);
+  }
+  flush();
+  finish<T>(sh, p, m, mc, s, w, p_ref, given, above, ref_tile);
+}
+
 // CTAs per row: enough for the GPU's resident CTAs (three per SM) when the rows alone are not, as long as
-// each still has a tile to read.
-static int choose_splits(long long rows, int vocab, int item, int sms) {
-  const long long tiles = ((long long)vocab * item + 16 * kTileWords - 1) / (16 * kTileWords);
-  int s = 1;
-  while (s < kMaxSplits && 2 * s <= tiles && rows * s * 2 <= (long long)kCtas * sms) s *= 2;
-  return s;
+// each still has kCtaBytes to read.
+constexpr int kCtaBytes = 16 * 1024;
+static int choose_log_splits(long long rows, int vocab, int item, int sms) {
+  const long long tiles = ((long long)vocab * item + kCtaBytes - 1) / kCtaBytes;
+  int log = 0;
+  while ((2 << log) <= kMaxSplits && (2 << log) <= tiles && (rows << (log + 1)) <= (long long)kCtas * sms) ++log;
+  return log;
 }
 
 template <typename T>
@@ -932,7 +1017,8 @@ extern "C" int neb_token_logprobs(const void* logits, int32_t dtype, int64_t row
   p.vocab = vocab;
   p.num_rows = num_rows;
   p.num_top = num_top;
-  p.splits = logprobs::choose_splits(num_rows, vocab, item, num_sms(dev));
+  p.log_splits = logprobs::choose_log_splits(num_rows, vocab, item, num_sms(dev));
+  p.splits = 1 << p.log_splits;
   p.token_ids = token_ids;
   p.logprobs = logprobs;
   p.ranks = ranks;
