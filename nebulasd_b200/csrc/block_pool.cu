@@ -2,18 +2,30 @@
 //
 // The pool is the callers': caches [num_blocks][layers * kv heads][block_size][head_dim], a block table
 // [rows][max_blocks] with the first seq_blocks[row] entries of a row in use, and one reference count per
-// block (0: free).  Every operator reads its lists on the device, so that a program which
-// chooses its branches on the device never waits for the host, and leaves the same result whatever the
-// order of its threads: blocks are taken lowest first, counts change by integer atomics.
+// block (0: free).  Every operator reads its lists on the device, so that a program which chooses its
+// branches on the device never waits for the host, and leaves the same result whatever the order of its
+// threads: blocks are taken lowest first, counts change by integer atomics.
 //
-// The simple form: plans by one CTA, copies with 16-byte loads and stores.
+// Fork and compact are two launches.  The plan is one thread-block cluster: its eight CTAs turn the
+// reference counts into a bitmap in shared memory, exchange their sums over distributed shared memory and so
+// give every free (or moved) block its rank without a grid-wide wait.  The second launch, which programmatic
+// serialisation brings up meanwhile, spreads tables and copies over the GPU.  A copy is bound by HBM (every byte
+// read and written once): a warp moves a 4 KB tile (one layer and head) at a time with up to eight 16-byte loads
+// per lane before the first store.
 #include "neb_common.cuh"
+#include "sm100.cuh"
 
 namespace neb {
 namespace blocks {
 
 constexpr int kPlanThreads = 1024;
+constexpr int kPlanWarps = kPlanThreads / 32;
+constexpr int kPlanCtas = 8;                       // one cluster
+constexpr long long kMaxPoolBlocks = 8ll << 20;    // a plan CTA's bitmap: 128 KB
 constexpr int kCopyThreads = 256;
+constexpr int kCopyWarps = kCopyThreads / 32;
+constexpr int kCopyCtas = 4;                       // resident per SM
+constexpr int kLoads = 8;                          // 16-byte loads per lane in flight
 
 struct Caches {
   char* plane[2];
@@ -36,7 +48,7 @@ __device__ __forceinline__ void report(unsigned int* bits, unsigned int bit) {
 
 // Exclusive prefix sum over the block's threads; `total` gets the sum.
 __device__ __forceinline__ int block_scan(int x, int* warp_sums, int& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int v = x;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -46,28 +58,55 @@ __device__ __forceinline__ int block_scan(int x, int* warp_sums, int& total) {
   __syncthreads();
   if (lane == 31) warp_sums[warp] = v;
   __syncthreads();
-  int before = 0, all = 0;
-  for (int i = 0; i < warps; ++i) {
-    const int s = warp_sums[i];
-    before += i < warp ? s : 0;
-    all += s;
-  }
-  total = all;
-  return before + v - x;
+  const int sum = warp_sums[lane];  // kPlanWarps == 32
+  total = __reduce_add_sync(~0u, sum);
+  return __reduce_add_sync(~0u, lane < warp ? sum : 0) + v - x;
+}
+static_assert(kPlanWarps == 32, "block_scan reads one sum per lane");
+
+// ------------------------------------------------------------- work of a warp
+// A warp copies a run of consecutive tiles out of all pairs' tiles, K plane before V plane.
+struct Run {
+  long long at, end;  // tile number: (pair * 2 + plane) * tiles + tile
+};
+__device__ __forceinline__ Run warp_run(long long tiles) {
+  const long long warps = (long long)gridDim.x * kCopyWarps, w = (long long)blockIdx.x * kCopyWarps + (threadIdx.x >> 5);
+  return Run{tiles * w / warps, tiles * (w + 1) / warps};
 }
 
-// Copies the first `tokens` tokens of every tile of [t0, t1) of one block and plane, by one CTA.
-__device__ __forceinline__ void copy_tiles(const Caches& c, int plane, long long src, long long dst, int tokens, int t0,
-                                           int t1) {
-  const int words = c.token_bytes / 16, pitch = c.block_size * words, live = tokens * words;
-  const long long block_words = (long long)c.tiles * pitch;
-  const uint4* s = reinterpret_cast<const uint4*>(c.plane[plane]) + src * block_words + (long long)t0 * pitch;
-  uint4* d = reinterpret_cast<uint4*>(c.plane[plane]) + dst * block_words + (long long)t0 * pitch;
-  const int n = (t1 - t0) * live;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    const int t = i / live;
-    const long long at = (long long)t * pitch + (i - t * live);
-    __stcs(d + at, __ldcs(s + at));
+// The first `live` of a tile's 16-byte words.
+__device__ __forceinline__ void copy_tile(const uint4* s, uint4* d, int live) {
+  const int lane = threadIdx.x & 31;
+  for (int base = lane; base < live; base += 32 * kLoads) {
+    uint4 v[kLoads];
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u)
+      if (base + 32 * u < live) v[u] = ld_stream_v4(s + base + 32 * u);
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u)
+      if (base + 32 * u < live) __stcs(d + base + 32 * u, v[u]);
+  }
+}
+
+// Copies the warp's run of `pairs` pairs' tiles.  pick(i, src, dst, tokens) looks a pair up (by the whole warp)
+// and says whether it is copied.
+template <typename Pick>
+__device__ __forceinline__ void copy_run(const Caches& c, int pairs, Pick pick) {
+  const int words = c.token_bytes / 16, pitch = c.block_size * words;
+  const Run run = warp_run(2ll * pairs * c.tiles);
+  long long at = run.at;
+  while (at < run.end) {
+    const long long plane_no = at / c.tiles;
+    const int tile = (int)(at - plane_no * c.tiles), pair = (int)(plane_no >> 1), plane = (int)(plane_no & 1);
+    const int n = (int)min((long long)(c.tiles - tile), run.end - at);
+    int src, dst, tokens;
+    if (pick(pair, src, dst, tokens)) {
+      const int live = tokens * words;
+      const uint4* s = reinterpret_cast<const uint4*>(c.plane[plane]) + ((long long)src * c.tiles + tile) * pitch;
+      uint4* d = reinterpret_cast<uint4*>(c.plane[plane]) + ((long long)dst * c.tiles + tile) * pitch;
+      for (int t = 0; t < n; ++t) copy_tile(s + (long long)t * pitch, d + (long long)t * pitch, live);
+    }
+    at += n;
   }
 }
 
@@ -78,38 +117,92 @@ struct CopyParams {
   const int32_t* dst;
   const int32_t* tokens;  // or null: whole blocks
   int n;
-  int chunk_tiles, chunks;  // tiles per work item, items per block and plane
   unsigned int* error_bits;
 };
 
-// One pair's checks, by the whole CTA: out of range, or in conflict with another pair.
-__device__ __forceinline__ bool pair_ok(const CopyParams& p, int i, int& src, int& dst, int& tokens) {
-  src = p.src[i];
-  dst = p.dst[i];
-  tokens = p.tokens ? p.tokens[i] : p.c.block_size;
-  unsigned int bad = 0;
-  if (src < 0 || src >= p.c.num_blocks || dst < 0 || dst >= p.c.num_blocks) bad |= kErrBlockIndex;
-  if (tokens < 0 || tokens > p.c.block_size) bad |= kErrInvalidRows;
-  bool clash = false;
-  for (int j = threadIdx.x; j < p.n; j += blockDim.x) {
-    const int other = p.dst[j];
-    clash |= j != i && (other == dst || other == src);
-  }
-  if (__syncthreads_or(clash)) bad |= kErrCopyConflict;
-  if (bad && threadIdx.x == 0) report(p.error_bits, bad);
-  return bad == 0 && src != dst;
+__global__ void __launch_bounds__(kCopyThreads, kCopyCtas) copy_kernel(const __grid_constant__ CopyParams p) {
+  copy_run(p.c, p.n, [&](int i, int& src, int& dst, int& tokens) {
+    src = p.src[i];
+    dst = p.dst[i];
+    tokens = p.tokens ? p.tokens[i] : p.c.block_size;
+    unsigned int bad = 0;
+    if (src < 0 || src >= p.c.num_blocks || dst < 0 || dst >= p.c.num_blocks) bad |= kErrBlockIndex;
+    if (tokens < 0 || tokens > p.c.block_size) bad |= kErrInvalidRows;
+    bool clash = false;
+    for (int j = threadIdx.x & 31; j < p.n; j += 32) {
+      const int other = p.dst[j];
+      clash |= j != i && (other == dst || other == src);
+    }
+    if (__any_sync(~0u, clash)) bad |= kErrCopyConflict;
+    if (bad && (threadIdx.x & 31) == 0) report(p.error_bits, bad);
+    return bad == 0 && src != dst;
+  });
 }
 
-__global__ void __launch_bounds__(kCopyThreads) copy_kernel(const CopyParams p) {
-  const long long items = 2ll * p.n * p.chunks;
-  for (long long it = blockIdx.x; it < items; it += gridDim.x) {
-    const int chunk = (int)(it % p.chunks);
-    const long long rest = it / p.chunks;
-    const int plane = (int)(rest & 1), pair = (int)(rest >> 1);
-    int src, dst, tokens;
-    if (!pair_ok(p, pair, src, dst, tokens)) continue;
-    const int t0 = chunk * p.chunk_tiles;
-    copy_tiles(p.c, plane, src, dst, tokens, t0, min(p.c.tiles, t0 + p.chunk_tiles));
+// ------------------------------------------------------------------------ plans
+// A plan CTA's part of the pool: blocks [first, first + count), a bit for each in `map`.
+struct PlanShared {
+  int sums[kPlanWarps];
+  int cta_bits[kPlanCtas];  // of every CTA of the cluster
+  int cta_more[kPlanCtas];
+  unsigned int map[1];      // (dynamic)
+};
+struct PlanPart {
+  long long first;
+  int count, words;
+};
+__device__ __forceinline__ PlanPart plan_part(long long num_blocks) {
+  const long long per = ((num_blocks + kPlanCtas * 32 - 1) / (kPlanCtas * 32)) * 32;
+  PlanPart r;
+  r.first = per * blockIdx.x;
+  r.count = (int)max(0ll, min(per, num_blocks - r.first));
+  r.words = (r.count + 31) / 32;
+  return r;
+}
+static size_t plan_smem(long long num_blocks) {
+  const long long per = ((num_blocks + kPlanCtas * 32 - 1) / (kPlanCtas * 32)) * 32;
+  return sizeof(PlanShared) + 4 * (size_t)(per / 32);
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// One int into every CTA's shared memory, at the place of this CTA.
+__device__ __forceinline__ void cluster_share(int* slots, int value) {
+  if (threadIdx.x < kPlanCtas) {
+    uint32_t to;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(sm100::smem_u32(slots + blockIdx.x)), "r"(threadIdx.x));
+    asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to), "r"(value) : "memory");
+  }
+}
+
+// Bits of the part's blocks whose count satisfies `bit`; returns how many (over the CTA).
+template <typename Bit>
+__device__ __forceinline__ int build_map(PlanShared& sh, const PlanPart& part, const int32_t* refs, Bit bit) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int mine = 0;
+#pragma unroll 4
+  for (int w = warp; w < part.words; w += kPlanWarps) {
+    const int i = 32 * w + lane;
+    const unsigned int word = __ballot_sync(~0u, i < part.count && bit(refs[part.first + i]));
+    if (lane == 0) sh.map[w] = word;
+    mine += __popc(word);
+  }
+  int total;
+  block_scan(lane == 0 ? mine : 0, sh.sums, total);
+  return total;
+}
+
+// fn(i, before) for every set bit i of the part, `before` set bits of the part before it.
+template <typename Fn>
+__device__ __forceinline__ void each_bit(PlanShared& sh, int words, Fn fn) {
+  int done = 0;
+  for (int base = 0; base < words; base += kPlanThreads) {
+    const int w = base + threadIdx.x;
+    unsigned int left = w < words ? sh.map[w] : 0u;
+    int all, before = block_scan(__popc(left), sh.sums, all);
+    for (before += done; left; left &= left - 1) fn(32 * w + __ffs(left) - 1, before++);
+    done += all;
   }
 }
 
@@ -125,20 +218,18 @@ struct ForkParams {
   int32_t* plan;   // [n][4]: shared blocks, all blocks (-1: refused), first of its slots, partial tokens
   int32_t* slots;  // free blocks, lowest first
   unsigned int* error_bits;
-  int chunk_tiles, chunks;
 };
 
-__global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParams p) {
-  __shared__ int sums[kPlanThreads / 32];
+// The children's shapes and their slots in order, by the first CTA; returns the slots needed.
+__device__ __forceinline__ int plan_children(const ForkParams& p, int* sums) {
   const int tid = threadIdx.x, bs = p.c.block_size;
-  // Each child's shape; nothing is written to the pool yet, so a row that is another child's parent is
-  // read as it was.
+  // Nothing is written to the pool yet, so a row that is another child's parent is read as it was.
   for (int i = tid; i < p.n; i += kPlanThreads) {
     const int parent = p.parents[i], child = p.children[i], len = p.lens[i];
-    const int cap = max(len, p.capacities ? p.capacities[i] : 0);
+    const int room = p.capacities ? p.capacities[i] : 0, cap = max(len, room);
     unsigned int bad = 0;
     if (child < 0 || child >= p.t.rows || (len > 0 && (parent < 0 || parent >= p.t.rows))) bad |= kErrSeqId;
-    if (len < 0 || (p.capacities && p.capacities[i] < 0)) bad |= kErrInvalidRows;
+    if (len < 0 || room < 0) bad |= kErrInvalidRows;
     const int shared = max(len, 0) / bs;
     const int total = (int)(((long long)max(cap, 0) + bs - 1) / bs);
     if (total > p.t.width) bad |= kErrTooManyBlocks;
@@ -161,8 +252,6 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParam
       report(p.error_bits, kErrInvalidRows);
       p.plan[4 * i + 1] = -1;
     }
-  __syncthreads();
-  // Slots in the children's order.
   int need = 0;
   for (int base = 0; base < p.n; base += kPlanThreads) {
     const int i = base + tid;
@@ -172,67 +261,97 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParam
     if (i < p.n) p.plan[4 * i + 2] = need + before;
     need += all;
   }
-  // The lowest free blocks.
-  int found = 0;
-  for (long long base = 0; base < p.c.num_blocks && found < need; base += kPlanThreads) {
-    const long long b = base + tid;
-    const int is_free = b < p.c.num_blocks && p.t.refs[b] == 0;
-    int all;
-    const int at = found + block_scan(is_free, sums, all);
-    if (is_free && at < need) p.slots[at] = (int)b;
-    found += all;
+  return need;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const __grid_constant__ ForkParams p) {
+  extern __shared__ __align__(16) unsigned char plan_raw[];
+  PlanShared& sh = *reinterpret_cast<PlanShared*>(plan_raw);
+  pdl_trigger();
+  const PlanPart part = plan_part(p.c.num_blocks);
+  asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+  const int is_free = build_map(sh, part, p.t.refs, [](int r) { return r == 0; });
+  const int need = blockIdx.x == 0 ? plan_children(p, sh.sums) : 0;
+  asm volatile("barrier.cluster.wait;" ::: "memory");  // every CTA has started
+  cluster_share(sh.cta_bits, is_free);
+  cluster_share(sh.cta_more, need);
+  cluster_sync();
+  const int wanted = sh.cta_more[0];
+  int before = 0, found = 0;
+  for (int i = 0; i < kPlanCtas; ++i) {
+    before += i < (int)blockIdx.x ? sh.cta_bits[i] : 0;
+    found += sh.cta_bits[i];
   }
-  for (int i = tid; i < p.n; i += kPlanThreads) {
-    const int total = p.plan[4 * i + 1];
-    if (total < 0) continue;
-    const int mine = total - p.plan[4 * i];
-    const bool granted = mine == 0 || p.plan[4 * i + 2] + mine <= found;
-    if (!granted) {
-      report(p.error_bits, kErrNoFreeBlock);
-      p.plan[4 * i + 1] = -1;
+  if (before < wanted)
+    each_bit(sh, part.words, [&](int i, int rank) {
+      if (before + rank < wanted) p.slots[before + rank] = (int)(part.first + i);
+    });
+  if (blockIdx.x == 0) {
+    for (int i = threadIdx.x; i < p.n; i += kPlanThreads) {
+      const int total = p.plan[4 * i + 1];
+      if (total < 0) continue;
+      const int mine = total - p.plan[4 * i];
+      const bool granted = mine == 0 || p.plan[4 * i + 2] + mine <= found;
+      if (!granted) {
+        report(p.error_bits, kErrNoFreeBlock);
+        p.plan[4 * i + 1] = -1;
+      }
+      p.t.seq_blocks[p.children[i]] = granted ? total : 0;
     }
-    p.t.seq_blocks[p.children[i]] = granted ? total : 0;
   }
 }
 
-__global__ void __launch_bounds__(kCopyThreads) fork_kernel(const ForkParams p) {
-  const long long items = 2ll * p.n * p.chunks;
-  for (long long it = blockIdx.x; it < items; it += gridDim.x) {
-    const int chunk = (int)(it % p.chunks);
-    const long long rest = it / p.chunks;
-    const int plane = (int)(rest & 1), i = (int)(rest >> 1);
-    const int shared = p.plan[4 * i], total = p.plan[4 * i + 1], slot = p.plan[4 * i + 2], part = p.plan[4 * i + 3];
-    if (total < 0) continue;
+constexpr int kEntries = 128;  // table entries that a warp takes at a time
+
+__global__ void __launch_bounds__(kCopyThreads, kCopyCtas) fork_kernel(const __grid_constant__ ForkParams p) {
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  // The children's rows.
+  const int per_row = (p.t.width + kEntries - 1) / kEntries;
+  const long long warps = (long long)gridDim.x * kCopyWarps;
+  for (long long unit = (long long)blockIdx.x * kCopyWarps + (threadIdx.x >> 5); unit < (long long)p.n * per_row;
+       unit += warps) {
+    const int i = (int)(unit / per_row), j0 = (int)(unit - (long long)i * per_row) * kEntries;
+    const int4 plan = reinterpret_cast<const int4*>(p.plan)[i];
+    const int shared = plan.x, total = plan.y;
+    if (j0 >= total) continue;
     const int32_t* from = p.t.table + (long long)p.parents[i] * p.t.width;
-    if (chunk == 0 && plane == 0) {
-      int32_t* to = p.t.table + (long long)p.children[i] * p.t.width;
-      for (int j = threadIdx.x; j < total; j += blockDim.x) {
-        int b;
-        if (j < shared) {
-          b = from[j];
-          if (b < 0 || b >= p.c.num_blocks) {
-            report(p.error_bits, kErrBlockIndex);
-            b = -1;
-          } else if (atomicAdd(&p.t.refs[b], 1) <= 0) {
-            report(p.error_bits, kErrRefCount);
-          }
-        } else {
-          b = p.slots[slot + j - shared];
-          p.t.refs[b] = 1;
-        }
-        to[j] = b;
-      }
+    int32_t* to = p.t.table + (long long)p.children[i] * p.t.width;
+    const int32_t* fresh = p.slots + plan.z - shared;
+    int b[kEntries / 32];
+#pragma unroll
+    for (int u = 0; u < kEntries / 32; ++u) {
+      const int j = j0 + lane + 32 * u;
+      b[u] = j < shared ? from[j] : j < total ? fresh[j] : -1;
     }
-    if (part > 0) {
-      const int src = from[shared];
-      if (src < 0 || src >= p.c.num_blocks) {
-        if (threadIdx.x == 0) report(p.error_bits, kErrBlockIndex);
-        continue;
+#pragma unroll
+    for (int u = 0; u < kEntries / 32; ++u) {
+      const int j = j0 + lane + 32 * u;
+      if (j >= total) break;
+      if (j < shared) {
+        if (b[u] < 0 || b[u] >= p.c.num_blocks) {
+          report(p.error_bits, kErrBlockIndex);
+          b[u] = -1;
+        } else if (atomicAdd(&p.t.refs[b[u]], 1) <= 0) {
+          report(p.error_bits, kErrRefCount);
+        }
+      } else {
+        p.t.refs[b[u]] = 1;
       }
-      const int t0 = chunk * p.chunk_tiles;
-      copy_tiles(p.c, plane, src, p.slots[slot], part, t0, min(p.c.tiles, t0 + p.chunk_tiles));
+      to[j] = b[u];
     }
   }
+  // The partial blocks.
+  copy_run(p.c, p.n, [&](int i, int& src, int& dst, int& tokens) {
+    const int4 plan = reinterpret_cast<const int4*>(p.plan)[i];
+    tokens = plan.w;
+    if (plan.y < 0 || tokens == 0) return false;
+    src = p.t.table[(long long)p.parents[i] * p.t.width + plan.x];
+    dst = p.slots[plan.z];
+    if (src >= 0 && src < p.c.num_blocks) return true;
+    if (lane == 0) report(p.error_bits, kErrBlockIndex);
+    return false;
+  });
 }
 
 // ------------------------------------------------------------------------ free
@@ -244,35 +363,51 @@ struct FreeParams {
   unsigned int* error_bits;
 };
 
-__global__ void __launch_bounds__(kCopyThreads) free_kernel(const FreeParams p) {
+// A CTA per row.  The first entries are loaded before the row's count is known.
+__global__ void __launch_bounds__(1024) free_kernel(const __grid_constant__ FreeParams p) {
   __shared__ int held;
+  constexpr int kAhead = 4;
   for (int i = blockIdx.x; i < p.n; i += gridDim.x) {
     const int row = p.list[i];
     if (row < 0 || row >= p.t.rows) {
       if (threadIdx.x == 0) report(p.error_bits, kErrSeqId);
       continue;
     }
-    __syncthreads();
-    // Whoever takes the count frees the row: one that is listed twice is freed once.
+    int32_t* entry = p.t.table + (long long)row * p.t.width;
+    int ahead[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int j = threadIdx.x + u * blockDim.x;
+      ahead[u] = j < p.t.width ? entry[j] : -1;
+    }
+    // Whoever takes the count frees the row: one that is listed twice is freed once.  (If it is, the entries
+    // above may be another CTA's -1 by now; then the count is 0 and they are not used.)
     if (threadIdx.x == 0) {
-      held = atomicExch(&p.t.seq_blocks[row], 0);
-      if (held < 0 || held > p.t.width) {
+      int n = atomicExch(&p.t.seq_blocks[row], 0);
+      if (n < 0 || n > p.t.width) {
         report(p.error_bits, kErrTooManyBlocks);
-        held = held < 0 ? 0 : p.t.width;
+        n = n < 0 ? 0 : p.t.width;
       }
+      held = n;
     }
     __syncthreads();
-    int32_t* entry = p.t.table + (long long)row * p.t.width;
-    for (int j = threadIdx.x; j < held; j += blockDim.x) {
-      const int b = entry[j];
+    const int n = held;
+    auto drop = [&](int j, int b) {
       entry[j] = -1;
       if (b < 0 || b >= p.num_blocks) {
         report(p.error_bits, kErrBlockIndex);
       } else if (atomicSub(&p.t.refs[b], 1) <= 0) {
-        atomicAdd(&p.t.refs[b], 1);  // it was free already: a count never stays negative
+        atomicAdd(&p.t.refs[b], 1);  // it was free already: a count never stays below what it was
         report(p.error_bits, kErrRefCount);
       }
+    };
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int j = threadIdx.x + u * blockDim.x;
+      if (j < n) drop(j, ahead[u]);
     }
+    for (int j = threadIdx.x + kAhead * blockDim.x; j < n; j += blockDim.x) drop(j, entry[j]);
+    __syncthreads();
   }
 }
 
@@ -285,69 +420,109 @@ struct CompactParams {
   int32_t* src;
   int32_t* dst;
   unsigned int* error_bits;
-  int chunk_tiles, chunks;
 };
 
-__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const CompactParams p) {
-  __shared__ int sums[kPlanThreads / 32];
-  const int tid = threadIdx.x;
-  const long long nb = p.c.num_blocks;
-  int mine = 0;
-  for (long long b = tid; b < nb; b += kPlanThreads) mine += p.t.refs[b] > 0;
-  int live;
-  block_scan(mine, sums, live);
-  // The i-th free block below `live` takes the i-th live block at or above it.
-  int holes = 0, movers = 0;
-  for (long long base = 0; base < nb; base += kPlanThreads) {
-    const long long b = base + tid;
-    const bool in = b < nb, used = in && p.t.refs[b] > 0;
-    const bool hole = in && !used && b < live, mover = used && b >= live;
-    int all_holes, all_movers;
-    const int ah = block_scan(hole, sums, all_holes), am = block_scan(mover, sums, all_movers);
-    if (hole) p.dst[holes + ah] = (int)b;
-    if (mover) p.src[movers + am] = (int)b;
-    if (in) p.new_index[b] = used ? (int)b : -1;
-    holes += all_holes;
-    movers += all_movers;
+__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const __grid_constant__ CompactParams p) {
+  extern __shared__ __align__(16) unsigned char plan_raw[];
+  PlanShared& sh = *reinterpret_cast<PlanShared*>(plan_raw);
+  pdl_trigger();
+  const PlanPart part = plan_part(p.c.num_blocks);
+  asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+  const int used = build_map(sh, part, p.t.refs, [](int r) { return r > 0; });
+  asm volatile("barrier.cluster.wait;" ::: "memory");  // every CTA has started
+  cluster_share(sh.cta_bits, used);
+  cluster_sync();
+  int live = 0, before = 0;  // blocks in use; those in earlier parts
+  for (int i = 0; i < kPlanCtas; ++i) {
+    before += i < (int)blockIdx.x ? sh.cta_bits[i] : 0;
+    live += sh.cta_bits[i];
   }
-  __syncthreads();
-  for (int i = tid; i < movers; i += kPlanThreads) {
-    const int s = p.src[i], d = p.dst[i];
-    p.new_index[s] = d;
-    p.t.refs[d] = p.t.refs[s];
-    p.t.refs[s] = 0;
+  // Blocks in use below index `live` stay.  Block `live` lies in one part, which knows how many those are.
+  const int low = (int)max(0ll, min((long long)part.count, live - part.first));  // the part's blocks below it
+  int stay = 0;
+  for (int w = threadIdx.x; w < part.words; w += kPlanThreads) {
+    const int bits = low - 32 * w;
+    stay += __popc(bits >= 32 ? sh.map[w] : bits > 0 ? sh.map[w] & ((1u << bits) - 1) : 0u);
   }
-  if (tid == 0) p.header[0] = movers;
+  int stay_part;
+  block_scan(stay, sh.sums, stay_part);
+  cluster_share(sh.cta_more, stay_part);
+  cluster_sync();
+  int stays = 0;
+  for (int i = 0; i < kPlanCtas; ++i) stays += sh.cta_more[i];
+  // The i-th free block below `live` takes the i-th block in use at or above it.
+  const int lane = threadIdx.x & 31;
+  int done = 0;
+  for (int base = 0; base < part.words; base += kPlanThreads) {
+    const int w0 = base + (int)(threadIdx.x & ~31);
+    const unsigned int word = w0 + lane < part.words ? sh.map[w0 + lane] : 0u;
+    int all;
+    const int mine = done + before + block_scan(__popc(word), sh.sums, all);  // in use before the word's blocks
+    done += all;
+    for (int q = 0; q < 32 && w0 + q < part.words; ++q) {  // a word per step, a block per lane
+      const unsigned int bits = __shfl_sync(~0u, word, q);
+      const int in_use = __shfl_sync(~0u, mine, q) + __popc(bits & ((1u << lane) - 1));
+      const int i = 32 * (w0 + q) + lane;
+      const long long b = part.first + i;
+      if (i >= part.count) continue;
+      const bool is_used = (bits >> lane) & 1;
+      p.new_index[b] = is_used ? (int)b : -1;  // (moved blocks get theirs below)
+      if (b < live) {
+        if (!is_used) p.dst[b - in_use] = (int)b;
+      } else if (is_used) {
+        p.src[in_use - stays] = (int)b;
+      }
+    }
+  }
+  const int moves = live - stays;
+  if (blockIdx.x == 0 && threadIdx.x == 0) p.header[0] = moves;
+  cluster_sync();
+  for (int i = blockIdx.x * kPlanThreads + threadIdx.x; i < moves; i += kPlanCtas * kPlanThreads)
+    p.new_index[__ldcg(p.src + i)] = __ldcg(p.dst + i);
 }
 
-__global__ void __launch_bounds__(kCopyThreads) compact_kernel(const CompactParams p) {
+__global__ void __launch_bounds__(kCopyThreads, kCopyCtas) compact_kernel(const __grid_constant__ CompactParams p) {
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
   // Table entries follow their blocks.
-  const long long entries = (long long)p.t.rows * p.t.width;
-  for (long long e = blockIdx.x * (long long)blockDim.x + threadIdx.x; e < entries;
-       e += (long long)gridDim.x * blockDim.x) {
-    const int row = (int)(e / p.t.width);
-    if (e - (long long)row * p.t.width >= p.t.seq_blocks[row]) continue;
-    const int b = p.t.table[e];
-    if (b < 0 || b >= p.c.num_blocks) {
-      report(p.error_bits, kErrBlockIndex);
-      continue;
+  const int per_row = (p.t.width + kEntries - 1) / kEntries;
+  const long long warps = (long long)gridDim.x * kCopyWarps;
+  for (long long unit = (long long)blockIdx.x * kCopyWarps + (threadIdx.x >> 5); unit < (long long)p.t.rows * per_row;
+       unit += warps) {
+    const int row = (int)(unit / per_row), j0 = (int)(unit - (long long)row * per_row) * kEntries;
+    const int held = min(p.t.seq_blocks[row], p.t.width);
+    if (j0 >= held) continue;
+    int32_t* entry = p.t.table + (long long)row * p.t.width + j0;
+    int b[kEntries / 32];
+#pragma unroll
+    for (int u = 0; u < kEntries / 32; ++u) b[u] = j0 + lane + 32 * u < held ? entry[lane + 32 * u] : -1;
+#pragma unroll
+    for (int u = 0; u < kEntries / 32; ++u) {
+      if (j0 + lane + 32 * u >= held) break;
+      if (b[u] < 0 || b[u] >= p.c.num_blocks) {
+        report(p.error_bits, kErrBlockIndex);
+        continue;
+      }
+      const int to = p.new_index[b[u]];
+      if (to < 0) report(p.error_bits, kErrRefCount);
+      if (to != b[u]) entry[lane + 32 * u] = to;
     }
-    const int to = p.new_index[b];
-    if (to < 0) report(p.error_bits, kErrRefCount);
-    if (to != b) p.t.table[e] = to;
   }
-  const long long items = 2ll * p.header[0] * p.chunks;
-  for (long long it = blockIdx.x; it < items; it += gridDim.x) {
-    const int chunk = (int)(it % p.chunks);
-    const long long rest = it / p.chunks;
-    const int plane = (int)(rest & 1), i = (int)(rest >> 1), t0 = chunk * p.chunk_tiles;
-    copy_tiles(p.c, plane, p.src[i], p.dst[i], p.c.block_size, t0, min(p.c.tiles, t0 + p.chunk_tiles));
+  // Blocks and counts.
+  const int moves = p.header[0];
+  for (int i = blockIdx.x * kCopyThreads + threadIdx.x; i < moves; i += gridDim.x * kCopyThreads) {
+    p.t.refs[p.dst[i]] = p.t.refs[p.src[i]];
+    p.t.refs[p.src[i]] = 0;
   }
+  copy_run(p.c, moves, [&](int i, int& src, int& dst, int& tokens) {
+    src = p.src[i];
+    dst = p.dst[i];
+    tokens = p.c.block_size;
+    return true;
+  });
 }
 
 // ------------------------------------------------------------------------ host
-constexpr int kChunkBytes = 64 * 1024;
-
 static int fill_caches(Caches& c, void* k, void* v, int64_t num_blocks, int32_t tiles, int32_t block_size,
                        int32_t token_bytes) {
   NEB_REQUIRE(num_blocks > 0 && num_blocks <= INT_MAX && tiles > 0 && block_size > 0, NEB_ERR_INVALID,
@@ -380,18 +555,45 @@ static int fill_tables(Tables& t, int32_t* table, int32_t rows, int32_t width, i
   return NEB_OK;
 }
 
-static void cut(const Caches& c, int& chunk_tiles, int& chunks) {
-  const int tile_bytes = c.block_size * c.token_bytes;
-  chunk_tiles = kChunkBytes / tile_bytes > 0 ? kChunkBytes / tile_bytes : 1;
-  chunks = (c.tiles + chunk_tiles - 1) / chunk_tiles;
-}
-
-static int copy_grid(long long items, unsigned& grid) {
+// CTAs for `units` warps of work, at most the resident ones.
+static int warp_grid(long long units, unsigned& grid) {
   int dev = 0;
   NEB_CUDA(cudaGetDevice(&dev));
-  const long long most = 8ll * num_sms(dev);
+  const long long most = (long long)kCopyCtas * num_sms(dev), ctas = (units + kCopyWarps - 1) / kCopyWarps;
   NEB_REQUIRE(most > 0, NEB_ERR_CUDA, "could not size the grid for device %d", dev);
-  grid = (unsigned)(items < most ? (items > 0 ? items : 1) : most);
+  grid = (unsigned)(ctas < 1 ? 1 : ctas < most ? ctas : most);
+  return NEB_OK;
+}
+
+static int check_plan_size(int64_t num_blocks) {
+  NEB_REQUIRE(num_blocks <= kMaxPoolBlocks, NEB_ERR_UNSUPPORTED, "pools of more than %lld blocks are not supported",
+              kMaxPoolBlocks);
+  return NEB_OK;
+}
+
+// A plan kernel as one cluster.
+template <typename P>
+static int launch_plan(void (*kernel)(const P), const P& p, cudaStream_t stream) {
+  static bool ready[64] = {};
+  int dev = 0;
+  NEB_CUDA(cudaGetDevice(&dev));
+  const size_t smem = plan_smem(p.c.num_blocks);
+  if (dev >= 64 || !ready[dev]) {
+    NEB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plan_smem(kMaxPoolBlocks)));
+    if (dev < 64) ready[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kPlanCtas);
+  cfg.blockDim = dim3(kPlanThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kPlanCtas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  NEB_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
   return NEB_OK;
 }
 
@@ -416,9 +618,8 @@ int neb_copy_blocks(void* k_cache, void* v_cache, int64_t num_blocks, int32_t ti
   p.tokens = num_tokens;
   p.n = num_pairs;
   p.error_bits = error_bits;
-  cut(p.c, p.chunk_tiles, p.chunks);
-  unsigned grid;
-  if (int rc = copy_grid(2ll * num_pairs * p.chunks, grid)) return rc;
+  unsigned grid = 1;
+  if (int rc = warp_grid(2ll * num_pairs * p.c.tiles, grid)) return rc;
   copy_kernel<<<grid, kCopyThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
   NEB_CUDA(cudaGetLastError());
   return NEB_OK;
@@ -438,6 +639,7 @@ int neb_fork_sequences(void* k_cache, void* v_cache, int64_t num_blocks, int32_t
   ForkParams p;
   if (int rc = fill_caches(p.c, k_cache, v_cache, num_blocks, tiles_per_block, block_size, token_bytes)) return rc;
   if (int rc = fill_tables(p.t, block_table, block_table_rows, max_blocks_per_seq, seq_blocks, ref_counts)) return rc;
+  if (int rc = check_plan_size(num_blocks)) return rc;
   NEB_REQUIRE(num_children >= 0, NEB_ERR_INVALID, "negative number of children");
   if (num_children == 0) return NEB_OK;
   NEB_REQUIRE(parents && children && seq_lens, NEB_ERR_INVALID, "null sequence list");
@@ -453,14 +655,12 @@ int neb_fork_sequences(void* k_cache, void* v_cache, int64_t num_blocks, int32_t
   p.plan = static_cast<int32_t*>(workspace);
   p.slots = p.plan + 4ll * num_children;
   p.error_bits = error_bits;
-  cut(p.c, p.chunk_tiles, p.chunks);
-  unsigned grid;
-  if (int rc = copy_grid(2ll * num_children * p.chunks, grid)) return rc;
+  unsigned grid = 1;
+  if (int rc = warp_grid(2ll * num_children * p.c.tiles + (long long)num_children * (p.t.width / kEntries + 1), grid))
+    return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  fork_plan_kernel<<<1, kPlanThreads, 0, s>>>(p);
-  NEB_CUDA(cudaGetLastError());
-  fork_kernel<<<grid, kCopyThreads, 0, s>>>(p);
-  NEB_CUDA(cudaGetLastError());
+  if (int rc = launch_plan(fork_plan_kernel, p, s)) return rc;
+  NEB_CUDA(launch_pdl(fork_kernel, dim3(grid), dim3(kCopyThreads), 0, s, p));
   return NEB_OK;
 }
 
@@ -477,9 +677,9 @@ int neb_free_sequences(int32_t* block_table, int32_t block_table_rows, int32_t m
   p.list = rows;
   p.n = num_rows;
   p.error_bits = error_bits;
-  unsigned grid;
-  if (int rc = copy_grid(num_rows, grid)) return rc;
-  free_kernel<<<grid, kCopyThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  // As many threads as one round over a row can use.
+  const int threads = max_blocks_per_seq <= 256 ? 256 : max_blocks_per_seq <= 512 ? 512 : 1024;
+  free_kernel<<<num_rows, threads, 0, static_cast<cudaStream_t>(stream)>>>(p);
   NEB_CUDA(cudaGetLastError());
   return NEB_OK;
 }
@@ -496,6 +696,7 @@ int neb_compact_blocks(void* k_cache, void* v_cache, int64_t num_blocks, int32_t
   CompactParams p;
   if (int rc = fill_caches(p.c, k_cache, v_cache, num_blocks, tiles_per_block, block_size, token_bytes)) return rc;
   if (int rc = fill_tables(p.t, block_table, block_table_rows, max_blocks_per_seq, seq_blocks, ref_counts)) return rc;
+  if (int rc = check_plan_size(num_blocks)) return rc;
   NEB_REQUIRE(new_index, NEB_ERR_INVALID, "new_index is null");
   NEB_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0 &&
                   workspace_bytes >= neb_compact_workspace_bytes(num_blocks),
@@ -506,14 +707,12 @@ int neb_compact_blocks(void* k_cache, void* v_cache, int64_t num_blocks, int32_t
   p.src = p.header + 4;
   p.dst = p.src + (num_blocks / 2 + 1);
   p.error_bits = error_bits;
-  cut(p.c, p.chunk_tiles, p.chunks);
-  unsigned grid;
-  if (int rc = copy_grid((num_blocks / 2 + 1) * 2ll * p.chunks, grid)) return rc;
+  unsigned grid = 1;
+  if (int rc = warp_grid(num_blocks / 2 * 2ll * p.c.tiles + (long long)p.t.rows * (p.t.width / kEntries + 1), grid))
+    return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  compact_plan_kernel<<<1, kPlanThreads, 0, s>>>(p);
-  NEB_CUDA(cudaGetLastError());
-  compact_kernel<<<grid, kCopyThreads, 0, s>>>(p);
-  NEB_CUDA(cudaGetLastError());
+  if (int rc = launch_plan(compact_plan_kernel, p, s)) return rc;
+  NEB_CUDA(launch_pdl(compact_kernel, dim3(grid), dim3(kCopyThreads), 0, s, p));
   return NEB_OK;
 }
 
