@@ -21,11 +21,19 @@ namespace blocks {
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
 constexpr int kPlanCtas = 8;                       // one cluster
-constexpr long long kMaxPoolBlocks = 8ll << 20;    // a plan CTA's bitmap: 128 KB
+constexpr int kMapCtas = kPlanCtas - 1;            // of a fork's plan: the first CTA has the children
+constexpr long long kMaxPoolBlocks = 8ll << 20;    // a plan CTA's bitmap: 147 KB at most
 constexpr int kCopyThreads = 256;
 constexpr int kCopyWarps = kCopyThreads / 32;
-constexpr int kCopyCtas = 4;                       // resident per SM
 constexpr int kLoads = 8;                          // 16-byte loads per lane in flight
+// Copies of whole blocks run two CTAs per SM: 64 KB of loads in flight per SM, then as many stores (more, and
+// reads and writes alternate in shorter runs: 512 blocks of 1.2 MB per plane 392 us, with four CTAs 415 us, with
+// one 519 us).  Items of 128 KB copy scattered pairs best (382 us; 64 KB 394, 32 KB 420), items of 32 KB the
+// ascending ones of a compaction (1.0 GB per plane 793 us; 64 KB 800, 128 KB 814).  Partial blocks have half the
+// loads in flight per warp: four CTAs, items of one tile per warp (64 partial blocks of 28 layers 24 us; with two
+// CTAs 27 us).
+constexpr int kWholeCtas = 2, kWholeTiles = 4 * kCopyWarps, kMoveTiles = kCopyWarps;
+constexpr int kPartCtas = 4, kPartTiles = kCopyWarps;
 
 struct Caches {
   char* plane[2];
@@ -64,16 +72,7 @@ __device__ __forceinline__ int block_scan(int x, int* warp_sums, int& total) {
 }
 static_assert(kPlanWarps == 32, "block_scan reads one sum per lane");
 
-// ------------------------------------------------------------- work of a warp
-// A warp copies a run of consecutive tiles out of all pairs' tiles, K plane before V plane.
-struct Run {
-  long long at, end;  // tile number: (pair * 2 + plane) * tiles + tile
-};
-__device__ __forceinline__ Run warp_run(long long tiles) {
-  const long long warps = (long long)gridDim.x * kCopyWarps, w = (long long)blockIdx.x * kCopyWarps + (threadIdx.x >> 5);
-  return Run{tiles * w / warps, tiles * (w + 1) / warps};
-}
-
+// ---------------------------------------------------------------------- copies
 // The first `live` of a tile's 16-byte words.
 __device__ __forceinline__ void copy_tile(const uint4* s, uint4* d, int live) {
   const int lane = threadIdx.x & 31;
@@ -88,25 +87,26 @@ __device__ __forceinline__ void copy_tile(const uint4* s, uint4* d, int live) {
   }
 }
 
-// Copies the warp's run of `pairs` pairs' tiles.  pick(i, src, dst, tokens) looks a pair up (by the whole warp)
-// and says whether it is copied.
-template <typename Pick>
-__device__ __forceinline__ void copy_run(const Caches& c, int pairs, Pick pick) {
-  const int words = c.token_bytes / 16, pitch = c.block_size * words;
-  const Run run = warp_run(2ll * pairs * c.tiles);
-  long long at = run.at;
-  while (at < run.end) {
-    const long long plane_no = at / c.tiles;
-    const int tile = (int)(at - plane_no * c.tiles), pair = (int)(plane_no >> 1), plane = (int)(plane_no & 1);
-    const int n = (int)min((long long)(c.tiles - tile), run.end - at);
+// Copies all pairs' tiles, K plane before V plane, in items of kTiles tiles of one block and plane that go round
+// the CTAs, a tile per warp: what the GPU reads and writes at a time stays a few tens of MB of neighbouring
+// tiles.  (A range of tiles per warp instead: 2 to 6 % slower.)  pick(i, src, dst, tokens) looks a pair up, called by
+// the whole CTA, and says whether it is copied.
+template <int kTiles, typename Pick>
+__device__ __forceinline__ void copy_pairs(const Caches& c, int pairs, Pick pick) {
+  const int words = c.token_bytes / 16, pitch = c.block_size * words, chunks = (c.tiles + kTiles - 1) / kTiles;
+  const long long items = 2ll * pairs * chunks;
+  for (long long it = blockIdx.x; it < items; it += gridDim.x) {
+    const long long plane_no = it / chunks;
+    const int tile = (int)(it - plane_no * chunks) * kTiles, pair = (int)(plane_no >> 1), plane = (int)(plane_no & 1);
+    const int n = min(kTiles, c.tiles - tile);
     int src, dst, tokens;
     if (pick(pair, src, dst, tokens)) {
       const int live = tokens * words;
       const uint4* s = reinterpret_cast<const uint4*>(c.plane[plane]) + ((long long)src * c.tiles + tile) * pitch;
       uint4* d = reinterpret_cast<uint4*>(c.plane[plane]) + ((long long)dst * c.tiles + tile) * pitch;
-      for (int t = 0; t < n; ++t) copy_tile(s + (long long)t * pitch, d + (long long)t * pitch, live);
+      for (int t = threadIdx.x >> 5; t < n; t += kCopyWarps)
+        copy_tile(s + (long long)t * pitch, d + (long long)t * pitch, live);
     }
-    at += n;
   }
 }
 
@@ -120,8 +120,9 @@ struct CopyParams {
   unsigned int* error_bits;
 };
 
-__global__ void __launch_bounds__(kCopyThreads, kCopyCtas) copy_kernel(const __grid_constant__ CopyParams p) {
-  copy_run(p.c, p.n, [&](int i, int& src, int& dst, int& tokens) {
+template <int kCtas, int kTiles>
+__global__ void __launch_bounds__(kCopyThreads, kCtas) copy_kernel(const __grid_constant__ CopyParams p) {
+  copy_pairs<kTiles>(p.c, p.n, [&](int i, int& src, int& dst, int& tokens) {
     src = p.src[i];
     dst = p.dst[i];
     tokens = p.tokens ? p.tokens[i] : p.c.block_size;
@@ -129,12 +130,12 @@ __global__ void __launch_bounds__(kCopyThreads, kCopyCtas) copy_kernel(const __g
     if (src < 0 || src >= p.c.num_blocks || dst < 0 || dst >= p.c.num_blocks) bad |= kErrBlockIndex;
     if (tokens < 0 || tokens > p.c.block_size) bad |= kErrInvalidRows;
     bool clash = false;
-    for (int j = threadIdx.x & 31; j < p.n; j += 32) {
+    for (int j = threadIdx.x; j < p.n; j += kCopyThreads) {
       const int other = p.dst[j];
       clash |= j != i && (other == dst || other == src);
     }
-    if (__any_sync(~0u, clash)) bad |= kErrCopyConflict;
-    if (bad && (threadIdx.x & 31) == 0) report(p.error_bits, bad);
+    if (__syncthreads_or(clash)) bad |= kErrCopyConflict;
+    if (bad && threadIdx.x == 0) report(p.error_bits, bad);
     return bad == 0 && src != dst;
   });
 }
@@ -151,16 +152,16 @@ struct PlanPart {
   long long first;
   int count, words;
 };
-__device__ __forceinline__ PlanPart plan_part(long long num_blocks) {
-  const long long per = ((num_blocks + kPlanCtas * 32 - 1) / (kPlanCtas * 32)) * 32;
+__device__ __forceinline__ PlanPart plan_part(long long num_blocks, int index, int parts) {
+  const long long per = ((num_blocks + parts * 32 - 1) / (parts * 32)) * 32;
   PlanPart r;
-  r.first = per * blockIdx.x;
+  r.first = per * index;
   r.count = (int)max(0ll, min(per, num_blocks - r.first));
   r.words = (r.count + 31) / 32;
   return r;
 }
-static size_t plan_smem(long long num_blocks) {
-  const long long per = ((num_blocks + kPlanCtas * 32 - 1) / (kPlanCtas * 32)) * 32;
+static size_t plan_smem(long long num_blocks, int parts) {
+  const long long per = ((num_blocks + parts * 32 - 1) / (parts * 32)) * 32;
   return sizeof(PlanShared) + 4 * (size_t)(per / 32);
 }
 
@@ -180,13 +181,23 @@ __device__ __forceinline__ void cluster_share(int* slots, int value) {
 template <typename Bit>
 __device__ __forceinline__ int build_map(PlanShared& sh, const PlanPart& part, const int32_t* refs, Bit bit) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int kAhead = 16;  // words of a warp whose counts are loaded before the first is used
   int mine = 0;
-#pragma unroll 4
-  for (int w = warp; w < part.words; w += kPlanWarps) {
-    const int i = 32 * w + lane;
-    const unsigned int word = __ballot_sync(~0u, i < part.count && bit(refs[part.first + i]));
-    if (lane == 0) sh.map[w] = word;
-    mine += __popc(word);
+  for (int w = warp; w < part.words; w += kAhead * kPlanWarps) {
+    int r[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = 32 * (w + u * kPlanWarps) + lane;
+      r[u] = i < part.count ? refs[part.first + i] : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int at = w + u * kPlanWarps;
+      if (at >= part.words) break;
+      const unsigned int word = __ballot_sync(~0u, 32 * at + lane < part.count && bit(r[u]));
+      if (lane == 0) sh.map[at] = word;
+      mine += __popc(word);
+    }
   }
   int total;
   block_scan(lane == 0 ? mine : 0, sh.sums, total);
@@ -220,45 +231,39 @@ struct ForkParams {
   unsigned int* error_bits;
 };
 
-// The children's shapes and their slots in order, by the first CTA; returns the slots needed.
-__device__ __forceinline__ int plan_children(const ForkParams& p, int* sums) {
-  const int tid = threadIdx.x, bs = p.c.block_size;
-  // Nothing is written to the pool yet, so a row that is another child's parent is read as it was.
-  for (int i = tid; i < p.n; i += kPlanThreads) {
-    const int parent = p.parents[i], child = p.children[i], len = p.lens[i];
-    const int room = p.capacities ? p.capacities[i] : 0, cap = max(len, room);
+// The children's shapes and their slots in order, by the first CTA, a child per thread and round: three round
+// trips to memory for up to 1,024 children.  Returns the slots needed; `last` is the thread's child of the last
+// round as written to p.plan.
+__device__ __forceinline__ int plan_children(const ForkParams& p, int* sums, int4& last) {
+  const int bs = p.c.block_size;
+  int need = 0;
+  for (int base = 0; base < p.n; base += kPlanThreads) {
+    const int i = base + threadIdx.x;
+    const bool in = i < p.n;
+    const int parent = in ? p.parents[i] : 0, child = in ? p.children[i] : 0, len = in ? p.lens[i] : 0;
+    const int room = in && p.capacities ? p.capacities[i] : 0;
     unsigned int bad = 0;
     if (child < 0 || child >= p.t.rows || (len > 0 && (parent < 0 || parent >= p.t.rows))) bad |= kErrSeqId;
     if (len < 0 || room < 0) bad |= kErrInvalidRows;
     const int shared = max(len, 0) / bs;
-    const int total = (int)(((long long)max(cap, 0) + bs - 1) / bs);
+    const int total = (int)(((long long)max(max(len, room), 0) + bs - 1) / bs);
     if (total > p.t.width) bad |= kErrTooManyBlocks;
-    if (!bad) {
-      if (p.t.seq_blocks[child] != 0) bad |= kErrInvalidRows;
-      if (len > 0 && ((long long)len + bs - 1) / bs > p.t.seq_blocks[parent]) bad |= kErrInvalidRows;
+    if (in && !bad) {
+      // Both rows as they were before the round's claims.  (A claim of an earlier round is negative: its row is
+      // neither empty nor long enough for a parent, as it would be refused within one round.)
+      const int held = __ldcg(&p.t.seq_blocks[child]), of_parent = len > 0 ? __ldcg(&p.t.seq_blocks[parent]) : 0;
+      if (held != 0 || (len > 0 && ((long long)len + bs - 1) / bs > of_parent)) bad |= kErrInvalidRows;
     }
-    if (bad) report(p.error_bits, bad);
-    p.plan[4 * i] = shared;
-    p.plan[4 * i + 1] = bad ? -1 : total;
-    p.plan[4 * i + 3] = max(len, 0) - shared * bs;
-  }
-  __syncthreads();
-  // A row listed twice goes to its first child: the lowest claim wins.
-  for (int i = tid; i < p.n; i += kPlanThreads)
-    if (p.plan[4 * i + 1] >= 0) atomicMin(&p.t.seq_blocks[p.children[i]], i - p.n);
-  __syncthreads();
-  for (int i = tid; i < p.n; i += kPlanThreads)
-    if (p.plan[4 * i + 1] >= 0 && __ldcg(&p.t.seq_blocks[p.children[i]]) != i - p.n) {
-      report(p.error_bits, kErrInvalidRows);
-      p.plan[4 * i + 1] = -1;
-    }
-  int need = 0;
-  for (int base = 0; base < p.n; base += kPlanThreads) {
-    const int i = base + tid;
-    const int mine = i < p.n && p.plan[4 * i + 1] >= 0 ? p.plan[4 * i + 1] - p.plan[4 * i] : 0;
+    __syncthreads();
+    // A row listed twice goes to its first child: the lowest claim wins.
+    if (in && !bad) atomicMin(&p.t.seq_blocks[child], i - p.n);
+    __syncthreads();
+    if (in && !bad && __ldcg(&p.t.seq_blocks[child]) != i - p.n) bad |= kErrInvalidRows;
+    if (in && bad) report(p.error_bits, bad);
     int all;
-    const int before = block_scan(mine, sums, all);
-    if (i < p.n) p.plan[4 * i + 2] = need + before;
+    const int before = block_scan(in && !bad ? total - shared : 0, sums, all);
+    last = make_int4(shared, bad ? -1 : total, need + before, max(len, 0) - shared * bs);
+    if (in) reinterpret_cast<int4*>(p.plan)[i] = last;
     need += all;
   }
   return need;
@@ -268,10 +273,18 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const __grid_co
   extern __shared__ __align__(16) unsigned char plan_raw[];
   PlanShared& sh = *reinterpret_cast<PlanShared*>(plan_raw);
   pdl_trigger();
-  const PlanPart part = plan_part(p.c.num_blocks);
   asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
-  const int is_free = build_map(sh, part, p.t.refs, [](int r) { return r == 0; });
-  const int need = blockIdx.x == 0 ? plan_children(p, sh.sums) : 0;
+  // The first CTA takes the children, the others the free blocks.
+  const bool first = blockIdx.x == 0;
+  PlanPart part{0, 0, 0};
+  int is_free = 0, need = 0;
+  int4 last = make_int4(0, -1, 0, 0);
+  if (first) {
+    need = plan_children(p, sh.sums, last);
+  } else {
+    part = plan_part(p.c.num_blocks, blockIdx.x - 1, kMapCtas);
+    is_free = build_map(sh, part, p.t.refs, [](int r) { return r == 0; });
+  }
   asm volatile("barrier.cluster.wait;" ::: "memory");  // every CTA has started
   cluster_share(sh.cta_bits, is_free);
   cluster_share(sh.cta_more, need);
@@ -282,28 +295,28 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const __grid_co
     before += i < (int)blockIdx.x ? sh.cta_bits[i] : 0;
     found += sh.cta_bits[i];
   }
-  if (before < wanted)
+  if (!first && before < wanted)
     each_bit(sh, part.words, [&](int i, int rank) {
       if (before + rank < wanted) p.slots[before + rank] = (int)(part.first + i);
     });
-  if (blockIdx.x == 0) {
+  if (first) {
     for (int i = threadIdx.x; i < p.n; i += kPlanThreads) {
-      const int total = p.plan[4 * i + 1];
-      if (total < 0) continue;
-      const int mine = total - p.plan[4 * i];
-      const bool granted = mine == 0 || p.plan[4 * i + 2] + mine <= found;
+      const int4 plan = p.n <= kPlanThreads ? last : reinterpret_cast<const int4*>(p.plan)[i];
+      if (plan.y < 0) continue;
+      const int mine = plan.y - plan.x;
+      const bool granted = mine == 0 || plan.z + mine <= found;
       if (!granted) {
         report(p.error_bits, kErrNoFreeBlock);
         p.plan[4 * i + 1] = -1;
       }
-      p.t.seq_blocks[p.children[i]] = granted ? total : 0;
+      p.t.seq_blocks[p.children[i]] = granted ? plan.y : 0;
     }
   }
 }
 
 constexpr int kEntries = 128;  // table entries that a warp takes at a time
 
-__global__ void __launch_bounds__(kCopyThreads, kCopyCtas) fork_kernel(const __grid_constant__ ForkParams p) {
+__global__ void __launch_bounds__(kCopyThreads, kPartCtas) fork_kernel(const __grid_constant__ ForkParams p) {
   pdl_wait();
   const int lane = threadIdx.x & 31;
   // The children's rows.
@@ -342,14 +355,14 @@ __global__ void __launch_bounds__(kCopyThreads, kCopyCtas) fork_kernel(const __g
     }
   }
   // The partial blocks.
-  copy_run(p.c, p.n, [&](int i, int& src, int& dst, int& tokens) {
+  copy_pairs<kPartTiles>(p.c, p.n, [&](int i, int& src, int& dst, int& tokens) {
     const int4 plan = reinterpret_cast<const int4*>(p.plan)[i];
     tokens = plan.w;
     if (plan.y < 0 || tokens == 0) return false;
     src = p.t.table[(long long)p.parents[i] * p.t.width + plan.x];
     dst = p.slots[plan.z];
     if (src >= 0 && src < p.c.num_blocks) return true;
-    if (lane == 0) report(p.error_bits, kErrBlockIndex);
+    if (threadIdx.x == 0) report(p.error_bits, kErrBlockIndex);
     return false;
   });
 }
@@ -426,7 +439,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const __grid
   extern __shared__ __align__(16) unsigned char plan_raw[];
   PlanShared& sh = *reinterpret_cast<PlanShared*>(plan_raw);
   pdl_trigger();
-  const PlanPart part = plan_part(p.c.num_blocks);
+  const PlanPart part = plan_part(p.c.num_blocks, blockIdx.x, kPlanCtas);
   asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
   const int used = build_map(sh, part, p.t.refs, [](int r) { return r > 0; });
   asm volatile("barrier.cluster.wait;" ::: "memory");  // every CTA has started
@@ -481,7 +494,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const __grid
     p.new_index[__ldcg(p.src + i)] = __ldcg(p.dst + i);
 }
 
-__global__ void __launch_bounds__(kCopyThreads, kCopyCtas) compact_kernel(const __grid_constant__ CompactParams p) {
+__global__ void __launch_bounds__(kCopyThreads, kWholeCtas) compact_kernel(const __grid_constant__ CompactParams p) {
   pdl_wait();
   const int lane = threadIdx.x & 31;
   // Table entries follow their blocks.
@@ -514,7 +527,7 @@ __global__ void __launch_bounds__(kCopyThreads, kCopyCtas) compact_kernel(const 
     p.t.refs[p.dst[i]] = p.t.refs[p.src[i]];
     p.t.refs[p.src[i]] = 0;
   }
-  copy_run(p.c, moves, [&](int i, int& src, int& dst, int& tokens) {
+  copy_pairs<kMoveTiles>(p.c, moves, [&](int i, int& src, int& dst, int& tokens) {
     src = p.src[i];
     dst = p.dst[i];
     tokens = p.c.block_size;
@@ -555,12 +568,14 @@ static int fill_tables(Tables& t, int32_t* table, int32_t rows, int32_t width, i
   return NEB_OK;
 }
 
-// CTAs for `units` warps of work, at most the resident ones.
-static int warp_grid(long long units, unsigned& grid) {
+// CTAs for a launch that copies up to `pairs` blocks and has `others` warps of other work.
+static int copy_grid(const Caches& c, int ctas_per_sm, int tiles, long long pairs, long long others, unsigned& grid) {
   int dev = 0;
   NEB_CUDA(cudaGetDevice(&dev));
-  const long long most = (long long)kCopyCtas * num_sms(dev), ctas = (units + kCopyWarps - 1) / kCopyWarps;
+  const long long most = (long long)ctas_per_sm * num_sms(dev);
   NEB_REQUIRE(most > 0, NEB_ERR_CUDA, "could not size the grid for device %d", dev);
+  const long long items = 2 * pairs * ((c.tiles + tiles - 1) / tiles), rest = (others + kCopyWarps - 1) / kCopyWarps;
+  const long long ctas = items > rest ? items : rest;
   grid = (unsigned)(ctas < 1 ? 1 : ctas < most ? ctas : most);
   return NEB_OK;
 }
@@ -577,9 +592,10 @@ static int launch_plan(void (*kernel)(const P), const P& p, cudaStream_t stream)
   static bool ready[64] = {};
   int dev = 0;
   NEB_CUDA(cudaGetDevice(&dev));
-  const size_t smem = plan_smem(p.c.num_blocks);
+  const size_t smem = plan_smem(p.c.num_blocks, kMapCtas);
   if (dev >= 64 || !ready[dev]) {
-    NEB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plan_smem(kMaxPoolBlocks)));
+    NEB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  (int)plan_smem(kMaxPoolBlocks, kMapCtas)));
     if (dev < 64) ready[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
@@ -619,8 +635,10 @@ int neb_copy_blocks(void* k_cache, void* v_cache, int64_t num_blocks, int32_t ti
   p.n = num_pairs;
   p.error_bits = error_bits;
   unsigned grid = 1;
-  if (int rc = warp_grid(2ll * num_pairs * p.c.tiles, grid)) return rc;
-  copy_kernel<<<grid, kCopyThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  if (int rc = copy_grid(p.c, num_tokens ? kPartCtas : kWholeCtas, num_tokens ? kPartTiles : kWholeTiles, num_pairs,
+                         0, grid)) return rc;
+  (num_tokens ? copy_kernel<kPartCtas, kPartTiles> : copy_kernel<kWholeCtas, kWholeTiles>)<<<grid, kCopyThreads, 0,
+                                                                   static_cast<cudaStream_t>(stream)>>>(p);
   NEB_CUDA(cudaGetLastError());
   return NEB_OK;
 }
@@ -656,8 +674,8 @@ int neb_fork_sequences(void* k_cache, void* v_cache, int64_t num_blocks, int32_t
   p.slots = p.plan + 4ll * num_children;
   p.error_bits = error_bits;
   unsigned grid = 1;
-  if (int rc = warp_grid(2ll * num_children * p.c.tiles + (long long)num_children * (p.t.width / kEntries + 1), grid))
-    return rc;
+  const long long rows = (long long)num_children * (p.t.width / kEntries + 1);
+  if (int rc = copy_grid(p.c, kPartCtas, kPartTiles, num_children, rows, grid)) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (int rc = launch_plan(fork_plan_kernel, p, s)) return rc;
   NEB_CUDA(launch_pdl(fork_kernel, dim3(grid), dim3(kCopyThreads), 0, s, p));
@@ -708,8 +726,8 @@ int neb_compact_blocks(void* k_cache, void* v_cache, int64_t num_blocks, int32_t
   p.dst = p.src + (num_blocks / 2 + 1);
   p.error_bits = error_bits;
   unsigned grid = 1;
-  if (int rc = warp_grid(num_blocks / 2 * 2ll * p.c.tiles + (long long)p.t.rows * (p.t.width / kEntries + 1), grid))
-    return rc;
+  const long long rows = (long long)p.t.rows * (p.t.width / kEntries + 1);
+  if (int rc = copy_grid(p.c, kWholeCtas, kMoveTiles, num_blocks / 2, rows, grid)) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (int rc = launch_plan(compact_plan_kernel, p, s)) return rc;
   NEB_CUDA(launch_pdl(compact_kernel, dim3(grid), dim3(kCopyThreads), 0, s, p));
