@@ -79,7 +79,7 @@ struct Shared {
   int first_index[kWarps];  // of each warp's range
   unsigned int tops[64];
   u64 threshold;  // only larger keys are listed; num_top listed ones are at or above it
-  float warp_f[3][kWarps];
+  float warp_f[4][kWarps];
   int warp_count[2][kWarps], warp_above[kWarps];
   int n;  // candidates offered (beyond kList: not all are listed)
 };
@@ -359,7 +359,7 @@ __device__ __forceinline__ void rank_keys(const u64* keys, int n, int num_top, u
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const u64 key = keys[i];
     int before = 0;
-#pragma unroll 4
+#pragma unroll 8
     for (int j = 0; j < n; ++j) before += keys[j] > key;
     if (key && before < num_top) sorted[before] = key;
   }
@@ -377,16 +377,17 @@ __device__ __forceinline__ bool list_candidates(Shared& sh, int from, int words,
   const unsigned int* piece_of = reinterpret_cast<const unsigned int*>(sh.slot[warp] + word) + (lane & 3);
   const int first = sh.first_index[warp] + from * kPer;
   const int every = k <= 8 ? 8 : k <= 16 ? 16 : 32;
+  const u64 thr = *static_cast<volatile u64*>(&sh.threshold);
+  if (*static_cast<volatile int*>(&sh.n) > kList) return false;
   bool due = false;
   auto offer = [&](float f, int idx) {
     const u64 key = make_key(f, idx);
-    if (key > *static_cast<volatile u64*>(&sh.threshold)) {
+    if (key > thr) {
       const int to = atomicAdd(&sh.n, 1);
       if (to < kList) sh.list[to] = key;
       due |= ((to + 1) & (every - 1)) == 0;
     }
   };
-  if (*static_cast<volatile int*>(&sh.n) > kList) return false;
   for (unsigned int left = __ballot_sync(~0u, cand); left; left &= left - 1) {
     const int other = __ffs(left) - 1;
     if (other + word < words) {
@@ -394,8 +395,10 @@ __device__ __forceinline__ bool list_candidates(Shared& sh, int from, int words,
       const int at = first + (other + word) * kPer + (lane & 3) * (kPer / 4);
       if constexpr (kPer == 8) {
         const float2 f = Elem<T>::pair(x);
-        if (f.x >= value) offer(f.x, at);
-        if (f.y >= value) offer(f.y, at + 1);
+        if (fmaxf(f.x, f.y) >= value) {
+          if (f.x >= value) offer(f.x, at);
+          if (f.y >= value) offer(f.y, at + 1);
+        }
       } else {
         if (__uint_as_float(x) >= value) offer(__uint_as_float(x), at);
       }
@@ -536,19 +539,23 @@ __device__ __noinline__ float tile_without(const uint4* data, int words, float M
   return sum;
 }
 
-// Joins `b` into `a`: sums about the larger maximum, which alone is left out of r.
-__device__ __forceinline__ Part join(Part a, Part b) {
-  if (b.m > a.m) {
-    const Part t = a;
-    a = b;
-    b = t;
-  }
-  const float dt = bounded((b.m - a.m) * kLog2e), f = fast_exp2(dt);
-  const float s = b.m == neg_inf() ? b.r : 1.f + b.r;  // b's maximum is an ordinary term now
-  a.r += f * s;
-  a.w += f * (b.w + s * dt);
-  a.above = ((a.above + b.above) & INT_MAX) | ((a.above | b.above) & kSkipped);
-  return a;
+// Joins the parts, one per lane of each warp (kMaxSplits at most): sums about the row's maximum, which alone is
+// left out of r.
+__device__ __forceinline__ Part join(const Part* parts, int n) {
+  const int lane = threadIdx.x & 31;
+  Part a = parts[lane < n ? lane : 0];
+  if (lane >= n) a = Part{neg_inf(), 0.f, 0.f, 0};
+  const float M = warp_max_nan(a.m);
+  const unsigned int top = __ballot_sync(~0u, a.m == M);
+  const float dt = bounded((a.m - M) * kLog2e), f = fast_exp2(dt);
+  const float own = a.m == neg_inf() || lane == __ffs(top) - 1 ? 0.f : 1.f;  // the part's maximum as an ordinary term
+  Part r;
+  r.m = M;
+  r.r = warp_sum(f * (own + a.r));
+  r.w = warp_sum(f * (a.w + (own + a.r) * dt));
+  const unsigned int skipped = __reduce_or_sync(~0u, (unsigned int)a.above) & (unsigned int)kSkipped;
+  r.above = __reduce_add_sync(~0u, a.above & INT_MAX) | (int)skipped;
+  return r;
 }
 
 // Any row, logit by logit, by one CTA: rows with a NaN or +inf (results NaN, order over all values) and rows
@@ -691,7 +698,19 @@ __device__ __noinline__ void finish(Shared& sh, const Params& p, float m, float 
       owner = other > M ? i : owner;
       M = fmaxf(M, other);
     }
-    if (owner == warp && M != neg_inf()) {
+    // The part's sum with its maximum, for a first look: from 2 on, subtracting the maximum's 1 loses nothing.
+    const float dt = bounded((m - M) * kLog2e), f = fast_exp2(dt), t0 = m == neg_inf() ? 0.f : exponent(m, mc),
+                inv = fast_exp2(-t0);
+    {
+      const float look = warp_sum(f * inv * (s + p_ref));
+      if (lane == 0) sh.warp_f[1][warp] = look;
+    }
+    __syncthreads();
+    float S = 0.f;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) S += sh.warp_f[1][i];
+    const bool apart = S < 2.f;
+    if (apart && owner == warp && M != neg_inf()) {
       // Sum the tile that holds the maximum again, without it.
       const float keep = p_ref != p_ref ? p_ref : 0.f;
       float rest = keep;
@@ -709,30 +728,31 @@ __device__ __noinline__ void finish(Shared& sh, const Params& p, float m, float 
     }
     // From the rounded reference to m, then to the CTA's maximum.  The maximum itself, left out of the owner's
     // sum, has a term in w: e0 t0.
-    const float t0 = m == neg_inf() ? 0.f : exponent(m, mc), inv = fast_exp2(-t0);
-    const float all = s + p_ref, q = (w - t0 * (all + (owner == warp && lane == 0 ? fast_exp2(t0) : 0.f))) * inv;
-    const float dt = bounded((m - M) * kLog2e), f = fast_exp2(dt);
-    const float r_sum = warp_sum(f * inv * all), w_sum = warp_sum(f * fmaf(inv * all, dt, q));
+    const float all = s + p_ref, left_out = apart && owner == warp && lane == 0 ? fast_exp2(t0) : 0.f;
+    const float q = (w - t0 * (all + left_out)) * inv;
+    const float r_sum = apart ? warp_sum(f * inv * all) : 0.f, w_sum = warp_sum(f * fmaf(inv * all, dt, q));
     const unsigned int skipped = __reduce_or_sync(~0u, (unsigned int)above) & (unsigned int)kSkipped;
     const int up = __reduce_add_sync(~0u, above & INT_MAX);
     if (lane == 0) {
-      sh.warp_f[1][warp] = r_sum;
+      if (apart) sh.warp_f[3][warp] = r_sum;
       sh.warp_f[2][warp] = w_sum;
       sh.warp_above[warp] = up | (int)skipped;
     }
     __syncthreads();
     if (k) {
       int n = sh.n;
-      if (n > kList) n = collect<T>(sh, at.data, at.words, at.index(0), at.x, p.vocab, part ? 0 : head, part ? 0 : tail, k);
+      if (n > kList)
+        n = collect<T>(sh, at.data, at.words, at.index(0), at.x, p.vocab, part ? 0 : head, part ? 0 : tail, k);
       rank_keys(sh.list, n, k, sh.sorted);
     }
     Part own{M, 0.f, 0.f, 0};
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) {
-      own.r += sh.warp_f[1][i];
+      own.r += apart ? sh.warp_f[3][i] : 0.f;
       own.w += sh.warp_f[2][i];
       own.above = ((own.above + sh.warp_above[i]) & INT_MAX) | ((own.above | sh.warp_above[i]) & kSkipped);
     }
+    if (!apart) own.r = S - 1.f;  // (NaN: apart is false, and stays NaN)
     if (splits == 1) {
       if (tid == 0) sh.parts[0] = own;
     } else {
@@ -759,8 +779,7 @@ __device__ __noinline__ void finish(Shared& sh, const Params& p, float m, float 
   const int tok = p.token_ids ? p.token_ids[row] : -1;
   const bool has_token = tok >= 0 && tok < p.vocab;
   if (tid == 0 && !has_token && tok != -1 && p.error_bits) atomicOr(p.error_bits, kErrTokenId);
-  Part a = sh.parts[0];
-  for (int i = 1; i < splits; ++i) a = join(a, sh.parts[i]);
+  Part a = splits > 1 ? join(sh.parts, splits) : sh.parts[0];
   if (a.r != a.r || a.w != a.w || a.m > kHighRow ||
       ((a.above & kSkipped) && !(a.m > kLowRow))) {
     general_row<T>(sh, p, at.x, row, has_token ? tok : -1);
@@ -893,7 +912,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const _
           for (int j = lane; j < all; j += 32) {
             const unsigned int own_top = sh.tops[j];
             int larger = 0, least = 0;
-#pragma unroll 4
+#pragma unroll 8
             for (int q = 0; q < all; ++q) {
               larger += sh.tops[q] > own_top;
               least += sh.tops[q] >= own_top;
