@@ -876,9 +876,9 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const _
       atomicOr(p.error_bits, kErrTimeout);
     // The given logit once a tile has been waited for: it is not waited for alone.
     if (from == 0 && tok >= 0 && tok < p.vocab) given = Elem<T>::load(at.x, tok);
-    // A whole tile lies in registers; of the last one, words are read as they are needed.
+    // A tile lies in registers; of a last one with few words, they are read as they are needed.
     const uint4* slot = sh.slot[warp];
-    const bool whole = nw >= kTileWords;
+    const bool whole = nw > kTileWords / 2;
     uint4 v[kWords];
     auto word = [&](int u, uint4 (&one)[1]) {
       const int a = lane + u * 32;
@@ -886,8 +886,17 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const _
     };
     float tm = neg_inf();
     if (whole) {
+      if (nw >= kTileWords) {
 #pragma unroll
-      for (int u = 0; u < kWords; ++u) v[u] = slot[lane + u * 32];
+        for (int u = 0; u < kWords; ++u) v[u] = slot[lane + u * 32];
+      } else {
+#pragma unroll
+        for (int u = 0; u < kWords; ++u) {
+          uint4 one[1];
+          word(u, one);
+          v[u] = one[0];
+        }
+      }
       tm = words_max<T>(v);
     } else {
       for (int u = 0; u * 32 < nw; ++u) {

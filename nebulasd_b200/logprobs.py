@@ -71,8 +71,8 @@ def _launch(logits, token_ids, num_top, rows, vocab, index) -> TokenLogprobs:
     logprobs = ranks = top_ids = top_logprobs = None
     entropy = torch.empty(rows, dtype=torch.float32, device=dev)
     if token_ids is not None:
-        logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
-        ranks = torch.empty(rows, dtype=torch.int32, device=dev)
+        logprobs = torch.empty_like(entropy)
+        ranks = torch.empty_like(token_ids)
     if num_top:
         top_ids = torch.empty((rows, num_top), dtype=torch.int32, device=dev)
         top_logprobs = torch.empty((rows, num_top), dtype=torch.float32, device=dev)
