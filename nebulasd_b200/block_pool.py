@@ -117,16 +117,18 @@ class BlockPool:
         self.k_cache, self.v_cache = k_cache, v_cache
         self.block_table, self.seq_blocks, self.ref_counts = block_table, seq_blocks, ref_counts
         self.num_blocks, self.block_size = shape[0], shape[2]
-        self._index = index
+        self._index, self._device = index, k_cache.device
         self._caches = (k_cache.data_ptr(), v_cache.data_ptr(), *shape)
         self._tables = (block_table.data_ptr(), *block_table.shape, seq_blocks.data_ptr(), ref_counts.data_ptr())
+        self._fork_bytes: dict[int, int] = {}
+        self._compact_bytes = _lib.lib.neb_compact_workspace_bytes(shape[0])
         self._word = new_error_word(index, "BlockPool")
         self._error_ptr = self._word.data_ptr()
 
     def _temporary(self, need: int) -> torch.Tensor:
         # From the caching allocator, so that calls on several streams and captured
         # graphs each have their own.
-        return torch.empty(need, dtype=torch.uint8, device=self.k_cache.device)
+        return torch.empty(need, dtype=torch.uint8, device=self._device)
 
     def fork(self, parents: torch.Tensor, children: torch.Tensor, seq_lens: torch.Tensor,
              capacities: torch.Tensor | None = None) -> None:
@@ -145,8 +147,10 @@ class BlockPool:
         _check_list("seq_lens", seq_lens, index, n)
         if capacities is not None:
             _check_list("capacities", capacities, index, n)
+        need = self._fork_bytes.get(n)
+        if need is None:
+            need = self._fork_bytes[n] = _lib.lib.neb_fork_workspace_bytes(self.num_blocks, n)
         with _Device(index):
-            need = _lib.lib.neb_fork_workspace_bytes(self.num_blocks, n)
             ws = self._temporary(need)
             rc = _lib.lib.neb_fork_sequences(*self._caches, *self._tables, parents.data_ptr(), children.data_ptr(),
                                              seq_lens.data_ptr(), _lib.ptr(capacities), n, ws.data_ptr(), need,
@@ -167,10 +171,10 @@ class BlockPool:
 
         Contents, counts and every row's entries move along.  Returns int32 ``[num_blocks]``: each block's
         new index (-1: it was free), for ids that the caller keeps elsewhere."""
+        need = self._compact_bytes
         with _Device(self._index):
-            need = _lib.lib.neb_compact_workspace_bytes(self.num_blocks)
             ws = self._temporary(need)
-            moved = torch.empty(self.num_blocks, dtype=torch.int32, device=self.k_cache.device)
+            moved = torch.empty_like(self.ref_counts)
             rc = _lib.lib.neb_compact_blocks(*self._caches, *self._tables, moved.data_ptr(), ws.data_ptr(), need,
                                              self._error_ptr, _raw_stream(self._index))
         _lib.check(rc, "compact")

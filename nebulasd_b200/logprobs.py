@@ -74,8 +74,8 @@ def _launch(logits, token_ids, num_top, rows, vocab, index) -> TokenLogprobs:
         logprobs = torch.empty_like(entropy)
         ranks = torch.empty_like(token_ids)
     if num_top:
-        top_ids = torch.empty((rows, num_top), dtype=torch.int32, device=dev)
         top_logprobs = torch.empty((rows, num_top), dtype=torch.float32, device=dev)
+        top_ids = torch.empty_like(top_logprobs, dtype=torch.int32)
     rc = _lib.lib.neb_token_logprobs(
         logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), vocab, rows, _lib.ptr(token_ids), num_top,
         _lib.ptr(logprobs), _lib.ptr(ranks), entropy.data_ptr(), _lib.ptr(top_ids), _lib.ptr(top_logprobs),
