@@ -13,16 +13,22 @@
 // A row is streamed by a cluster of S CTAs (S = 1 when the rows alone fill the
 // GPU), each warp through a 4 KB tile of shared memory that a bulk asynchronous
 // copy fills while the tile before is summed from registers.  No warp waits for
-// another, and the row is read once.  The CTAs leave
-// their sums and candidates in the first CTA's shared memory, so there is no
-// workspace and no second launch.
+// another, and the row is read once.  The CTAs leave their sums and candidates in
+// the first CTA's shared memory, so there is no workspace and no second launch.
 //
 // Alternatives: a CTA keeps a list of candidates and a threshold that num_top of
 // them reach.  A lane compares its tile maximum (needed for m anyway) with the
 // threshold, and only where it is higher does the warp look at that lane's logits
 // again, in the tile, and list those above it.  The warp that lists every 8th (16th,
-// 32nd: by num_top) candidate raises the threshold.  So after the first tile a tile costs one
-// comparison and now and then a candidate, and no barrier.
+// 32nd: by num_top) candidate raises the threshold.  So after the first tile a tile
+// costs one comparison, now and then a candidate, and no barrier: 2,048 rows of
+// 151,936 fp16 logits list about 22 each for 5 alternatives, 90 for 20.
+//
+// What bounds it: HBM for many rows (2,048 of them: 110 us without alternatives,
+// 5.7 TB/s, 125 us with 5, 152 us with 20; reading them alone in this way takes
+// 105 us), with the XU pipe's exp2 (one per logit, 69 us) and about 8 instructions
+// per logit behind it.  For few rows, latency: one row 6.5 us, with 20 alternatives
+// 11.5 us, of which the launch, the first tile and the joins are all but 2 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -40,11 +46,11 @@ constexpr int kCtas = 3;                   // resident per SM
 constexpr int kMaxTop = NEB_MAX_TOP_LOGPROBS;
 constexpr int kMaxSplits = 8;              // CTAs per row (the portable cluster size)
 constexpr int kList = 512;                 // candidates
-constexpr int kWindow = 128;               // the last candidates, among which it is looked for
+constexpr int kWindow = 128;               // the last candidates, which a higher threshold is taken from
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr uint32_t kWaitNs = 20000;                // a tile's wait: kWaitTries times this, 2 s
-constexpr int kWaitTries = 100000;
+constexpr uint32_t kWaitNs = 20000;        // of sleep between two looks at a tile
+constexpr long long kWaitLimit = 4000000000ll;  // cycles (about 2 s)
 
 typedef unsigned long long u64;
 
@@ -301,11 +307,16 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-// Bounded (about 2 s), asleep between tries: the other CTAs' warps need the issue slots.
+// The warp's wait for its tile: bounded, asleep between looks (the other warps need the issue slots).
 __device__ __forceinline__ bool wait_full(uint64_t* bar, uint32_t parity) {
-  for (int i = 0; i < kWaitTries; ++i)
-    if (sm100::mbar_try_wait_sleep(bar, parity, kWaitNs)) return true;
-  return false;
+  bool ok = sm100::mbar_try_wait_sleep(bar, parity, kWaitNs);
+  if (!ok) {
+    const long long t0 = clock64();
+    do {
+      ok = sm100::mbar_try_wait_sleep(bar, parity, kWaitNs);
+    } while (!ok && clock64() - t0 < kWaitLimit);
+  }
+  return __all_sync(~0u, ok);
 }
 
 // ------------------------------------------------------------ block reductions
@@ -326,8 +337,8 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// The largest threshold search: a key `lo` with lowest <= #(keys > lo) <= most among the block's keys
-// (mine(i) for i < mine_n, at least `lowest` of them above `lo` on entry).  Keys differ, so it exists.
+// A key `lo` with lowest <= #(keys > lo) <= most among the block's keys (mine(i) for i < mine_n, more than `most`
+// of them above `lo` on entry).  Keys differ, so it exists.
 template <typename F>
 __device__ __forceinline__ u64 search(Shared& sh, int& turn, u64 lo, int lowest, int most, int mine_n, F mine) {
   u64 top = 0;
@@ -482,18 +493,46 @@ __device__ __noinline__ int collect(Shared& sh, const uint4* data, int words, in
 }
 
 // Fills `sorted` from n to k with the logits below kLow, which the candidates leave out: largest first (all of
-// them mostly equal, -inf or another mask), then by index.
+// them mostly equal, -inf or another mask), then by index.  A pass over the row for the next lower value, four
+// words per thread in flight, and its first logits.
 template <typename T>
-__device__ __noinline__ void fill_masked(Shared& sh, u64* sorted, const void* x, int vocab, int n, int k) {
-  const int tid = threadIdx.x;
+__device__ __noinline__ void fill_masked(Shared& sh, u64* sorted, const void* x, int vocab, int head, int n, int k) {
+  constexpr int kPer = Elem<T>::kPerWord;
+  const int tid = threadIdx.x, words = (vocab - head) / kPer;
+  const uint4* data = reinterpret_cast<const uint4*>(static_cast<const T*>(x) + head);
   int turn = 0;
   float limit = kLow;
   while (n < k) {
-    unsigned int best = 0;
-    for (int j = tid; j < vocab; j += kThreads) {
-      const float v = Elem<T>::load(x, j);
-      if (v < limit) best = max(best, order_f32(v));
+    float next = neg_inf();
+    bool any = false;
+    auto look = [&](float v) {
+      if (v < limit) {
+        next = fmaxf(next, v);
+        any = true;
+      }
+    };
+    for (int base = tid; base < words; base += 4 * kThreads) {
+      uint4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (base + u * kThreads < words) v[u] = __ldg(data + base + u * kThreads);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (base + u * kThreads >= words) break;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if constexpr (kPer == 8) {
+            const float2 f = Elem<T>::pair(piece(v[u], q));
+            look(f.x);
+            look(f.y);
+          } else {
+            look(__uint_as_float(piece(v[u], q)));
+          }
+        }
+      }
     }
+    for (int j = tid; j < vocab - words * kPer; j += kThreads) look(Elem<T>::load(x, j < head ? j : j + words * kPer));
+    unsigned int best = any ? order_f32(next) : 0u;
     best = __reduce_max_sync(~0u, best);
     __syncthreads();
     if ((tid & 31) == 0) sh.warp_key[tid >> 5] = best;
@@ -730,8 +769,7 @@ __device__ __noinline__ void finish(Shared& sh, const Params& p, float m, float 
     const bool apart = S < 2.f;
     if (apart && owner == warp && M != neg_inf()) {
       // Sum the tile that holds the maximum again, without it.
-      const float keep = p_ref != p_ref ? p_ref : 0.f;
-      float rest = keep;
+      float rest = p_ref != p_ref ? p_ref : 0.f;
       int equal = 0;  // logits equal to the maximum
       if (ref_tile < 0) {
         equal = lone == M;
@@ -798,8 +836,7 @@ __device__ __noinline__ void finish(Shared& sh, const Params& p, float m, float 
   const bool has_token = tok >= 0 && tok < p.vocab;
   if (tid == 0 && !has_token && tok != -1 && p.error_bits) atomicOr(p.error_bits, kErrTokenId);
   Part a = splits > 1 ? join(sh.parts, splits) : sh.parts[0];
-  if (a.r != a.r || a.w != a.w || a.m > kHighRow ||
-      ((a.above & kSkipped) && !(a.m > kLowRow))) {
+  if (a.r != a.r || a.w != a.w || a.m > kHighRow || ((a.above & kSkipped) && !(a.m > kLowRow))) {
     general_row<T>(sh, p, at.x, row, has_token ? tok : -1);
     return;
   }
@@ -809,7 +846,7 @@ __device__ __noinline__ void finish(Shared& sh, const Params& p, float m, float 
     int listed = 0;
     while (top_keys[listed]) ++listed;
     __syncthreads();
-    fill_masked<T>(sh, top_keys, at.x, p.vocab, listed, k);
+    fill_masked<T>(sh, top_keys, at.x, p.vocab, head, listed, k);
   }
   const float nan = __int_as_float(0x7fffffff);
   const float ln_s = a.m == neg_inf() ? nan : log1pf(a.r);
@@ -847,11 +884,14 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const _
   if (p.splits > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
   const int tok = p.token_ids ? p.token_ids[at.row] : -1;
   float given = __int_as_float(0x7f800000);
-  for (int i = tid; i < kList; i += kThreads) sh.list[i] = 0;
-  if (tid < kMaxTop) sh.sorted[tid] = sh.merged[tid] = 0;
-  if (tid == 0) {
-    sh.n = 0;
-    sh.threshold = ((u64)order_f32(kLow) << 32) - 1;  // masked logits are no candidates
+  if (k) {
+    for (int i = tid; i < kList; i += kThreads) sh.list[i] = 0;
+    if (tid < kMaxTop) sh.sorted[tid] = sh.merged[tid] = 0;
+    if (tid == 0) {
+      sh.n = 0;
+      sh.threshold = ((u64)order_f32(kLow) << 32) - 1;  // masked logits are no candidates
+    }
+    if (lane == 0) sh.first_index[warp] = at.index(at.first_word());
   }
   __syncwarp();
 
@@ -868,12 +908,11 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const _
     w += b.x + b.y;
     acc_s = acc_w = 0;
   };
-  if (lane == 0) sh.first_index[warp] = at.index(at.first_word());
-  __syncwarp();
-  for (int from = 0; from == 0 || from < mine; from += kTileWords) {
+  bool lost = false;  // a tile never came: the row is wrong, and the warp asks for no more
+  for (int from = 0; from == 0 || (from < mine && !lost); from += kTileWords) {
     const int nw = mine - from;  // words from this tile on
-    if (nw > 0 && !wait_full(&sh.full[warp], (from / kTileWords) & 1) && p.error_bits)
-      atomicOr(p.error_bits, kErrTimeout);
+    if (nw > 0 && !wait_full(&sh.full[warp], (from / kTileWords) & 1))
+      lost = !wait_full(&sh.full[warp], (from / kTileWords) & 1);  // (once more: the copy may be under way)
     // The given logit once a tile has been waited for: it is not waited for alone.
     if (from == 0 && tok >= 0 && tok < p.vocab) given = Elem<T>::load(at.x, tok);
     // A tile lies in registers; of a last one with few words, they are read as they are needed.
@@ -956,7 +995,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const _
       if (__any_sync(~0u, cand)) due = list_candidates<T>(sh, from, nw, cand, thr_value, k);
     }
     __syncwarp();  // the slot is read
-    if (lane == 0 && from + kTileWords < mine) fill(from + kTileWords);
+    if (lane == 0 && from + kTileWords < mine && !lost) fill(from + kTileWords);
 
     // ---- sums, while the next tiles arrive
     const bool raise = top > m && top >= kLow;
@@ -998,6 +1037,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const _
     if (due) raise_threshold(sh, k);
   }
   flush();
+  if (lost && lane == 0 && p.error_bits) atomicOr(p.error_bits, kErrTimeout);
   finish<T>(sh, p, m, mc, s, w, p_ref, given, above, ref_tile);
 }
 

@@ -126,6 +126,7 @@ def test_masks(dtype, cuda):
     base[9, :15000] = -inf                 # whole tiles banned
     base[10, :] = torch.finfo(dtype).max   # all at the highest
     base[11, 3] = torch.finfo(dtype).max
+    base[9, [100, 14000]] = low            # (and two masked otherwise)
     tokens = torch.tensor([2, 19000, 4, 200, 9, 7, 11, 11, 4, 14, 3, 4], dtype=torch.int32, device=cuda)
     for k in (0, 6, 32):
         got = _check(base.to(dtype).to(cuda), tokens, k)
@@ -149,6 +150,22 @@ def test_confident_rows_keep_their_precision(dtype, rows, cuda):
         a, b = a.double().cpu(), torch.as_tensor(b)
         assert bool(((a - b).abs() <= 4 * g * b.abs()).all())
     assert got.ranks.tolist() == rk.tolist() and got.top_ids.tolist() == ids.tolist()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 30, 500])
+def test_fewer_allowed_tokens_than_alternatives(dtype, rows, cuda):
+    """A grammar's mask: a few tokens left, some ruled out by the lowest value, the others by -inf."""
+    vocab = 12345
+    g = torch.Generator().manual_seed(rows)
+    x = torch.full((rows, vocab), -math.inf)
+    for r in range(rows):
+        at = torch.randperm(vocab, generator=g)
+        x[r, at[:r % 9]] = torch.randn(r % 9, generator=g)
+        x[r, at[10:10 + r % 5]] = torch.finfo(dtype).min
+        if r % 3 == 0:
+            x[r, at[20:40]] = -66000.0 if dtype != torch.float16 else -65250.0
+    _check(x.to(dtype).to(cuda), torch.randint(0, vocab, (rows,), generator=g).to(torch.int32).to(cuda), 20)
 
 
 def test_row_splits_give_one_answer(cuda):
