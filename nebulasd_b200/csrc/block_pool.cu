@@ -87,26 +87,33 @@ __device__ __forceinline__ void copy_tile(const uint4* s, uint4* d, int live) {
   }
 }
 
+struct Pair {
+  int src, dst, tokens;
+};
+
 // Copies all pairs' tiles, K plane before V plane, in items of kTiles tiles of one block and plane that go round
 // the CTAs, a tile per warp: what the GPU reads and writes at a time stays a few tens of MB of neighbouring
-// tiles.  (A range of tiles per warp instead: 2 to 6 % slower.)  pick(i, src, dst, tokens) looks a pair up, called by
-// the whole CTA, and says whether it is copied.
-template <int kTiles, typename Pick>
-__device__ __forceinline__ void copy_pairs(const Caches& c, int pairs, Pick pick) {
+// tiles.  (A range of tiles per warp instead: 2 to 6 % slower.)  load(i) fetches a pair, for the next item while
+// this one is copied; keep(i, pair), called by the whole CTA, says whether it is copied.
+template <int kTiles, typename Load, typename Keep>
+__device__ __forceinline__ void copy_pairs(const Caches& c, int pairs, Load load, Keep keep) {
   const int words = c.token_bytes / 16, pitch = c.block_size * words, chunks = (c.tiles + kTiles - 1) / kTiles;
   const long long items = 2ll * pairs * chunks;
-  for (long long it = blockIdx.x; it < items; it += gridDim.x) {
+  long long it = blockIdx.x;
+  if (it >= items) return;
+  Pair next = load((int)(it / chunks >> 1));
+  while (it < items) {
+    const Pair pair = next;
     const long long plane_no = it / chunks;
-    const int tile = (int)(it - plane_no * chunks) * kTiles, pair = (int)(plane_no >> 1), plane = (int)(plane_no & 1);
-    const int n = min(kTiles, c.tiles - tile);
-    int src, dst, tokens;
-    if (pick(pair, src, dst, tokens)) {
-      const int live = tokens * words;
-      const uint4* s = reinterpret_cast<const uint4*>(c.plane[plane]) + ((long long)src * c.tiles + tile) * pitch;
-      uint4* d = reinterpret_cast<uint4*>(c.plane[plane]) + ((long long)dst * c.tiles + tile) * pitch;
-      for (int t = threadIdx.x >> 5; t < n; t += kCopyWarps)
-        copy_tile(s + (long long)t * pitch, d + (long long)t * pitch, live);
-    }
+    const int tile = (int)(it - plane_no * chunks) * kTiles, plane = (int)(plane_no & 1);
+    it += gridDim.x;
+    if (it < items) next = load((int)(it / chunks >> 1));
+    if (!keep((int)(plane_no >> 1), pair)) continue;
+    const int n = min(kTiles, c.tiles - tile), live = pair.tokens * words;
+    const uint4* s = reinterpret_cast<const uint4*>(c.plane[plane]) + ((long long)pair.src * c.tiles + tile) * pitch;
+    uint4* d = reinterpret_cast<uint4*>(c.plane[plane]) + ((long long)pair.dst * c.tiles + tile) * pitch;
+    for (int t = threadIdx.x >> 5; t < n; t += kCopyWarps)
+      copy_tile(s + (long long)t * pitch, d + (long long)t * pitch, live);
   }
 }
 
@@ -122,22 +129,23 @@ struct CopyParams {
 
 template <int kCtas, int kTiles>
 __global__ void __launch_bounds__(kCopyThreads, kCtas) copy_kernel(const __grid_constant__ CopyParams p) {
-  copy_pairs<kTiles>(p.c, p.n, [&](int i, int& src, int& dst, int& tokens) {
-    src = p.src[i];
-    dst = p.dst[i];
-    tokens = p.tokens ? p.tokens[i] : p.c.block_size;
-    unsigned int bad = 0;
-    if (src < 0 || src >= p.c.num_blocks || dst < 0 || dst >= p.c.num_blocks) bad |= kErrBlockIndex;
-    if (tokens < 0 || tokens > p.c.block_size) bad |= kErrInvalidRows;
-    bool clash = false;
-    for (int j = threadIdx.x; j < p.n; j += kCopyThreads) {
-      const int other = p.dst[j];
-      clash |= j != i && (other == dst || other == src);
-    }
-    if (__syncthreads_or(clash)) bad |= kErrCopyConflict;
-    if (bad && threadIdx.x == 0) report(p.error_bits, bad);
-    return bad == 0 && src != dst;
-  });
+  const int own = (int)threadIdx.x < p.n ? p.dst[threadIdx.x] : -1;  // the thread's share of the first destinations
+  copy_pairs<kTiles>(
+      p.c, p.n,
+      [&](int i) { return Pair{p.src[i], p.dst[i], p.tokens ? p.tokens[i] : p.c.block_size}; },
+      [&](int i, const Pair& a) {
+        unsigned int bad = 0;
+        if (a.src < 0 || a.src >= p.c.num_blocks || a.dst < 0 || a.dst >= p.c.num_blocks) bad |= kErrBlockIndex;
+        if (a.tokens < 0 || a.tokens > p.c.block_size) bad |= kErrInvalidRows;
+        bool clash = (int)threadIdx.x < p.n && (int)threadIdx.x != i && (own == a.dst || own == a.src);
+        for (int j = threadIdx.x + kCopyThreads; j < p.n; j += kCopyThreads) {
+          const int other = p.dst[j];
+          clash |= j != i && (other == a.dst || other == a.src);
+        }
+        if (__syncthreads_or(clash)) bad |= kErrCopyConflict;
+        if (bad && threadIdx.x == 0) report(p.error_bits, bad);
+        return bad == 0 && a.src != a.dst;
+      });
 }
 
 // ------------------------------------------------------------------------ plans
@@ -354,17 +362,23 @@ __global__ void __launch_bounds__(kCopyThreads, kPartCtas) fork_kernel(const __g
       to[j] = b[u];
     }
   }
-  // The partial blocks.
-  copy_pairs<kPartTiles>(p.c, p.n, [&](int i, int& src, int& dst, int& tokens) {
+  // The partial blocks.  A pair takes three loads that depend on each other: once per CTA for the first children.
+  auto look_up = [&](int i) {
     const int4 plan = reinterpret_cast<const int4*>(p.plan)[i];
-    tokens = plan.w;
-    if (plan.y < 0 || tokens == 0) return false;
-    src = p.t.table[(long long)p.parents[i] * p.t.width + plan.x];
-    dst = p.slots[plan.z];
-    if (src >= 0 && src < p.c.num_blocks) return true;
-    if (threadIdx.x == 0) report(p.error_bits, kErrBlockIndex);
-    return false;
-  });
+    if (plan.y < 0 || plan.w == 0) return Pair{-1, -1, 0};
+    return Pair{p.t.table[(long long)p.parents[i] * p.t.width + plan.x], p.slots[plan.z], plan.w};
+  };
+  __shared__ Pair known[kCopyThreads];
+  if ((int)threadIdx.x < p.n) known[threadIdx.x] = look_up(threadIdx.x);
+  __syncthreads();
+  copy_pairs<kPartTiles>(
+      p.c, p.n, [&](int i) { return i < kCopyThreads ? known[i] : look_up(i); },
+      [&](int, const Pair& a) {
+        if (a.tokens == 0) return false;
+        if (a.src >= 0 && a.src < p.c.num_blocks) return true;
+        if (threadIdx.x == 0) report(p.error_bits, kErrBlockIndex);
+        return false;
+      });
 }
 
 // ------------------------------------------------------------------------ free
@@ -527,12 +541,8 @@ __global__ void __launch_bounds__(kCopyThreads, kWholeCtas) compact_kernel(const
     p.t.refs[p.dst[i]] = p.t.refs[p.src[i]];
     p.t.refs[p.src[i]] = 0;
   }
-  copy_pairs<kMoveTiles>(p.c, moves, [&](int i, int& src, int& dst, int& tokens) {
-    src = p.src[i];
-    dst = p.dst[i];
-    tokens = p.c.block_size;
-    return true;
-  });
+  copy_pairs<kMoveTiles>(
+      p.c, moves, [&](int i) { return Pair{p.src[i], p.dst[i], p.c.block_size}; }, [](int, const Pair&) { return true; });
 }
 
 // ------------------------------------------------------------------------ host
