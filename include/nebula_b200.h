@@ -213,8 +213,9 @@ int neb_greedy_accept(const void* logits, int64_t row_stride, int32_t vocab, int
  * -inf logits (banned tokens) have probability 0.  A row that holds a NaN or
  * +inf, or nothing but -inf, gets NaN for every floating result; its order is
  * still defined (a NaN counts as the largest value, -0 equals +0).  A token
- * outside [-1, vocab) is treated as -1 and recorded as bit 6 of *error_bits.
- * Needs no workspace. */
+ * outside [-1, vocab) is treated as -1 and recorded as bit 6 of *error_bits
+ * (device memory, optional; bit 3: a bounded wait gave up, the row is wrong).
+ * Needs no workspace, keeps nothing between calls. */
 #define NEB_DTYPE_F16 0
 #define NEB_DTYPE_BF16 1
 #define NEB_DTYPE_F32 2
@@ -321,7 +322,8 @@ int neb_rotary_inplace(void* q, void* k, const void* cos, const void* sin, int32
  * max_blocks_per_seq, bit 4 invalid rows, lengths or token counts, bit 7 a block
  * in use without a positive count, bit 8 too few free blocks, bit 9 copies in
  * conflict.  Calls on one pool must be ordered; no list may be part of the pool's
- * tables, and the tables may not overlap. */
+ * tables, and the tables may not overlap.  Fork and compact take pools of up to
+ * 2^23 blocks. */
 
 /* Block dst[i] gets the first num_tokens[i] tokens (null: all) of block src[i],
  * all tiles, both planes; the rest of dst[i] keeps its contents.  A pair whose

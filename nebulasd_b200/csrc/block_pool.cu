@@ -27,11 +27,11 @@ constexpr int kCopyThreads = 256;
 constexpr int kCopyWarps = kCopyThreads / 32;
 constexpr int kLoads = 8;                          // 16-byte loads per lane in flight
 // Copies of whole blocks run two CTAs per SM: 64 KB of loads in flight per SM, then as many stores (more, and
-// reads and writes alternate in shorter runs: 512 blocks of 1.2 MB per plane 392 us, with four CTAs 415 us, with
-// one 519 us).  Items of 128 KB copy scattered pairs best (382 us; 64 KB 394, 32 KB 420), items of 32 KB the
-// ascending ones of a compaction (1.0 GB per plane 793 us; 64 KB 800, 128 KB 814).  Partial blocks have half the
-// loads in flight per warp: four CTAs, items of one tile per warp (64 partial blocks of 28 layers 24 us; with two
-// CTAs 27 us).
+// reads and writes alternate in shorter runs: 512 blocks of 1.2 MB per plane in items of 64 KB 392 us, with four
+// CTAs 415 us, with one 519 us).  Items of 128 KB copy scattered pairs best (383 us, 6.3 TB/s; 64 KB 395, 32 KB
+// 420), items of 32 KB the ascending ones of a compaction (2.4 GB moved, 768 us; 64 KB 777, 128 KB 786).  Partial
+// blocks have half the loads in flight per warp: four CTAs, items of one tile per warp (64 partial blocks of 28
+// layers 24 us, 5.2 TB/s; with two CTAs 27 us, with two tiles per warp 25 us).
 constexpr int kWholeCtas = 2, kWholeTiles = 4 * kCopyWarps, kMoveTiles = kCopyWarps;
 constexpr int kPartCtas = 4, kPartTiles = kCopyWarps;
 
@@ -93,8 +93,8 @@ struct Pair {
 
 // Copies all pairs' tiles, K plane before V plane, in items of kTiles tiles of one block and plane that go round
 // the CTAs, a tile per warp: what the GPU reads and writes at a time stays a few tens of MB of neighbouring
-// tiles.  (A range of tiles per warp instead: 2 to 6 % slower.)  load(i) fetches a pair, for the next item while
-// this one is copied; keep(i, pair), called by the whole CTA, says whether it is copied.
+// tiles.  (A range of tiles per warp instead: 2 to 6 % slower.)  load(i) fetches a pair, for the next item before
+// this one is copied (3 % of a compaction); keep(i, pair), called by the whole CTA, says whether it is copied.
 template <int kTiles, typename Load, typename Keep>
 __device__ __forceinline__ void copy_pairs(const Caches& c, int pairs, Load load, Keep keep) {
   const int words = c.token_bytes / 16, pitch = c.block_size * words, chunks = (c.tiles + kTiles - 1) / kTiles;
@@ -542,7 +542,8 @@ __global__ void __launch_bounds__(kCopyThreads, kWholeCtas) compact_kernel(const
     p.t.refs[p.src[i]] = 0;
   }
   copy_pairs<kMoveTiles>(
-      p.c, moves, [&](int i) { return Pair{p.src[i], p.dst[i], p.c.block_size}; }, [](int, const Pair&) { return true; });
+      p.c, moves, [&](int i) { return Pair{p.src[i], p.dst[i], p.c.block_size}; },
+      [](int, const Pair&) { return true; });
 }
 
 // ------------------------------------------------------------------------ host

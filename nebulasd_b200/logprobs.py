@@ -86,5 +86,5 @@ def _launch(logits, token_ids, num_top, rows, vocab, index) -> TokenLogprobs:
 
 def workspace_errors(device: torch.device | None = None) -> int:
     """Synchronise the device's current stream and return (and clear) the error bits that
-    calls on it recorded (bit 6: a token outside ``[-1, vocab)``)."""
+    calls on it recorded (bit 6: a token outside ``[-1, vocab)``; bit 3: a bounded wait gave up)."""
     return _errors.read(device)

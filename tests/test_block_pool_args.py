@@ -72,6 +72,15 @@ def test_bad_lists_and_workspaces():
     assert L.neb_compact_workspace_bytes(0) == L.neb_compact_workspace_bytes(2 ** 31) == 0
 
 
+def test_pools_beyond_the_plan():
+    """Fork and compact plan pools of up to 2^23 blocks."""
+    big, ws = 2 ** 23 + 1, 1 << 40
+    assert L.neb_fork_sequences(*_caches(nb=big, tiles=1, size=1, token=16), *_tables(), A, A, A, None, 1, A, ws, None,
+                                None) == _lib.NEB_ERR_UNSUPPORTED
+    assert L.neb_compact_blocks(*_caches(nb=big, tiles=1, size=1, token=16), *_tables(), A, A, ws, None,
+                                None) == _lib.NEB_ERR_UNSUPPORTED
+
+
 def test_host_tensors_are_refused():
     k = torch.zeros((4, 1, 1, 16, 128), dtype=torch.float16)
     i = torch.zeros(1, dtype=torch.int32)
