@@ -7,6 +7,10 @@ Ops (``nebulasd_b200.kernels``), with the reference's names and signatures:
   * ``rmsnorm_inplace``          RMSNorm (Qwen3 QK-norm)
   * ``qk_norm_rope_store``       the last three fused into one launch
   * ``flash_attn_varlen_func``   causal prefill attention (verify kernel, no host sync)
+After the forward (``nebulasd_b200.accept``, ``nebulasd_b200.logprobs``):
+``greedy_accept`` and ``token_logprobs`` of the logits, without a host sync.
+Branching (``nebulasd_b200.block_pool``): ``copy_blocks``, and ``BlockPool`` to
+fork, free and compact sequences that share cache blocks.
 HostKV (``nebulasd_b200.hostkv``): ``NativeCopyBackend`` for restore/writeback,
 ``migrate_blocks`` for same-role peer migration.
 

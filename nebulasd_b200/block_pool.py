@@ -55,7 +55,8 @@ def copy_blocks(k_cache: torch.Tensor, v_cache: torch.Tensor, src: torch.Tensor,
     once, so a pair whose ``dst`` is another pair's ``dst``, or whose ``src`` is
     another pair's ``dst``, is left out and reported by ``workspace_errors``
     (bit 9), as is one with a block (bit 0) or token count (bit 4) out of range.
-    Runs on the current stream of the caches' device.
+    Runs on the current stream of the caches' device; its first call on a device
+    must come before any graph capture.
     """
     nb, tiles, size, token_bytes = _check_caches(k_cache, v_cache)
     index, n = k_cache.get_device(), src.shape[0] if src.dim() else 0

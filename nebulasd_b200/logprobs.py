@@ -42,7 +42,8 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor | None = None, 
     the lowest id.  Sums are fp32.  Banned tokens (-inf) have probability 0; a
     row with a NaN, a +inf or nothing but -inf gets NaN results.  A token
     outside ``[-1, vocab)`` counts as -1 and is reported by ``workspace_errors``
-    (bit 6).  Runs on the current stream of the logits' device.
+    (bit 6).  Runs on the current stream of the logits' device; its first call on
+    a device must come before any graph capture.
     """
     if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in _DTYPES:
         raise ValueError("logits must be a [rows, vocab] tensor of float16, bfloat16 or float32")
