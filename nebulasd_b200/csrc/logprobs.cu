@@ -47,6 +47,7 @@ constexpr int kMaxTop = NEB_MAX_TOP_LOGPROBS;
 constexpr int kMaxSplits = 8;              // CTAs per row (the portable cluster size)
 constexpr int kList = 512;                 // candidates
 constexpr int kWindow = 128;               // the last candidates, which a higher threshold is taken from
+constexpr int kMaxVocab = 1 << 30;         // (an index in int with tiles to spare)
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr uint32_t kWaitNs = 20000;        // of sleep between two looks at a tile
@@ -122,6 +123,8 @@ __device__ __forceinline__ float key_value(u64 key) { return value_of_order((uns
 // large negative number) are never a reference: beside such a maximum their share is exp(-1000) or less.
 constexpr float kLow = -65000.f, kLowRow = -64000.f, kHighRow = 66000.f;
 constexpr float kFinite = -65504.f;
+// The threshold below every key but those of such masked logits.
+__device__ __forceinline__ u64 no_masked() { return ((u64)order_f32(kLow) << 32) - 1; }
 
 template <>
 struct Elem<__half> {
@@ -448,16 +451,15 @@ __device__ __noinline__ void raise_threshold(Shared& sh, int num_top) {
   if (best && lane == 0) atomicMax(&sh.threshold, ((u64)best << 32) | 0xffffffffu);
 }
 
-// The candidates of a row part whose list ran over (equal or rising logits), word by word from memory: the
-// num_top largest, in sh.list.  Returns how many.
+// The num_top largest keys above `thr` of a row part whose list ran over (equal or rising logits) or of a whole row,
+// word by word from memory: in order in sh.list.  Returns how many.
 template <typename T>
 __device__ __noinline__ int collect(Shared& sh, const uint4* data, int words, int first, const void* x, int vocab,
-                                    int head, int tail, int k) {
+                                    int head, int tail, int k, u64 thr) {
   constexpr int kPer = Elem<T>::kPerWord;
   constexpr int kMost = kThreads - kMaxTop;
   const int tid = threadIdx.x;
   int turn = 0, n = 0;
-  u64 thr = ((u64)order_f32(kLow) << 32) - 1;
   for (int base = 0; base == 0 || base < words; base += kThreads) {
     u64 key[kPer + 1] = {};
     if (base + tid < words) {
@@ -615,9 +617,11 @@ __device__ __forceinline__ Part join(const Part* parts, int n) {
 }
 
 // Any row, logit by logit, by one CTA: rows with a NaN or +inf (results NaN, order over all values) and rows
-// that have nothing above kLow.
+// that have nothing above kLow.  Slow, as such rows are rare: a wholly masked row of 151,936 fp16 logits 44 us, with
+// 20 alternatives 103 us (their largest in one pass of keys; a pass per alternative took 619 us), beside the 12 us
+// and 20 us of a call for another row.
 template <typename T>
-__device__ __noinline__ void general_row(Shared& sh, const Params& p, const void* x, int row, int tok) {
+__device__ __noinline__ void general_row(Shared& sh, const Params& p, const void* x, int row, int head, int tok) {
   const int tid = threadIdx.x;
   const float nan = __int_as_float(0x7fffffff);
   int turn = 0, above = 0;
@@ -658,27 +662,16 @@ __device__ __noinline__ void general_row(Shared& sh, const Params& p, const void
     if (p.ranks) p.ranks[row] = tok >= 0 ? 1 + above : 0;
     if (p.entropy) p.entropy[row] = ln_s - kLn2 * (w / s);
   }
-  u64 limit = ~0ull;
-  for (int k = 0; k < p.num_top; ++k) {
-    u64 best = 0;
-    for (int j = tid; j < p.vocab; j += kThreads) {
-      const u64 key = make_key(Elem<T>::load(x, j), j);
-      if (key < limit && key > best) best = key;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const u64 n = __shfl_xor_sync(~0u, best, o);
-      best = n > best ? n : best;
-    }
-    __syncthreads();
-    if ((tid & 31) == 0) sh.warp_key[tid >> 5] = best;
-    __syncthreads();
-    limit = 0;
-    for (int i = 0; i < kWarps; ++i) limit = sh.warp_key[i] > limit ? sh.warp_key[i] : limit;
-    if (tid == 0) {
-      p.top_ids[(long long)row * p.num_top + k] = key_index(limit);
-      p.top_logprobs[(long long)row * p.num_top + k] = (key_value(limit) - m) - ln_s;
-    }
+  const int k = p.num_top;
+  if (k == 0) return;
+  constexpr int kPer = Elem<T>::kPerWord;
+  const int words = (p.vocab - head) / kPer, tail = p.vocab - head - words * kPer;
+  const uint4* data = reinterpret_cast<const uint4*>(static_cast<const T*>(x) + head);
+  collect<T>(sh, data, words, head, x, p.vocab, head, tail, k, 0);  // (every key is above 0)
+  if (tid < k) {
+    const u64 key = sh.list[tid];
+    p.top_ids[(long long)row * k + tid] = key_index(key);
+    p.top_logprobs[(long long)row * k + tid] = (key_value(key) - m) - ln_s;
   }
 }
 
@@ -798,7 +791,8 @@ __device__ __noinline__ void finish(Shared& sh, const Params& p, float m, float 
     if (k) {
       int n = sh.n;
       if (n > kList)
-        n = collect<T>(sh, at.data, at.words, at.index(0), at.x, p.vocab, part ? 0 : head, part ? 0 : tail, k);
+        n = collect<T>(sh, at.data, at.words, at.index(0), at.x, p.vocab, part ? 0 : head, part ? 0 : tail, k,
+                       no_masked());
       rank_keys(sh.list, n, k, sh.sorted);
     }
     Part own{M, 0.f, 0.f, 0};
@@ -837,7 +831,7 @@ __device__ __noinline__ void finish(Shared& sh, const Params& p, float m, float 
   if (tid == 0 && !has_token && tok != -1 && p.error_bits) atomicOr(p.error_bits, kErrTokenId);
   Part a = splits > 1 ? join(sh.parts, splits) : sh.parts[0];
   if (a.r != a.r || a.w != a.w || a.m > kHighRow || ((a.above & kSkipped) && !(a.m > kLowRow))) {
-    general_row<T>(sh, p, at.x, row, has_token ? tok : -1);
+    general_row<T>(sh, p, at.x, row, head, has_token ? tok : -1);
     return;
   }
   a.above &= INT_MAX;
@@ -889,7 +883,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const _
     if (tid < kMaxTop) sh.sorted[tid] = sh.merged[tid] = 0;
     if (tid == 0) {
       sh.n = 0;
-      sh.threshold = ((u64)order_f32(kLow) << 32) - 1;  // masked logits are no candidates
+      sh.threshold = no_masked();
     }
     if (lane == 0) sh.first_index[warp] = at.index(at.first_word());
   }
@@ -1086,6 +1080,8 @@ extern "C" int neb_token_logprobs(const void* logits, int32_t dtype, int64_t row
   NEB_REQUIRE(dtype == NEB_DTYPE_F16 || dtype == NEB_DTYPE_BF16 || dtype == NEB_DTYPE_F32, NEB_ERR_INVALID,
               "unknown logits dtype %d", dtype);
   NEB_REQUIRE(num_rows >= 0 && vocab > 0 && row_stride >= 0, NEB_ERR_INVALID, "invalid sizes");
+  NEB_REQUIRE(vocab <= logprobs::kMaxVocab, NEB_ERR_UNSUPPORTED, "rows of more than %d logits are not supported",
+              logprobs::kMaxVocab);
   NEB_REQUIRE(num_top >= 0 && num_top <= vocab && num_top <= NEB_MAX_TOP_LOGPROBS, NEB_ERR_INVALID,
               "num_top %d outside [0, min(vocab, %d)]", num_top, NEB_MAX_TOP_LOGPROBS);
   if (num_rows == 0) return NEB_OK;

@@ -42,7 +42,7 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor | None = None, 
     the lowest id.  Sums are fp32.  Banned tokens (-inf) have probability 0; a
     row with a NaN, a +inf or nothing but -inf gets NaN results.  A token
     outside ``[-1, vocab)`` counts as -1 and is reported by ``workspace_errors``
-    (bit 6).  Runs on the current stream of the logits' device; its first call on
+    (bit 6).  No gradients.  Runs on the current stream of the logits' device; its first call on
     a device must come before any graph capture.
     """
     if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in _DTYPES:
@@ -51,8 +51,8 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor | None = None, 
     index = logits.get_device()
     if index < 0:
         raise ValueError("logits must be on a CUDA device")
-    if vocab == 0:
-        raise ValueError("logits need a vocabulary")
+    if not 0 < vocab <= 1 << 30 or rows >= 1 << 31:
+        raise ValueError("logits need 1 to 2^30 logits per row and fewer than 2^31 rows")
     if vocab > 1 and logits.stride(1) != 1:
         raise ValueError("logits must have contiguous rows")
     if token_ids is not None:

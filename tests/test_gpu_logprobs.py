@@ -168,6 +168,31 @@ def test_fewer_allowed_tokens_than_alternatives(dtype, rows, cuda):
     _check(x.to(dtype).to(cuda), torch.randint(0, vocab, (rows,), generator=g).to(torch.int32).to(cuda), 20)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,offset", [(1, 0), (9, 3), (480, 5)])
+def test_rows_without_a_finite_share(dtype, rows, offset, cuda):
+    """Rows with a NaN or +inf and wholly masked ones among others, by one CTA and by several."""
+    vocab = 12007
+    x, tokens = _logits(rows, rows, vocab + offset, dtype, "cpu")
+    tokens = (tokens % vocab).to(cuda)
+    low = torch.finfo(dtype).min
+    for i in range(0, rows, 3):
+        kind = (i // 3) % 5
+        if kind == 0:
+            x[i] = low
+            x[i, ::7] = -math.inf
+        elif kind == 1:
+            x[i, 5 + 11 * i::400] = math.nan
+        elif kind == 2:
+            x[i, -1] = math.inf
+        elif kind == 3:
+            x[i] = math.nan
+        else:
+            x[i] = -70000. - torch.arange(vocab + offset) if dtype != torch.float16 else low
+    for k in (1, 20, 32):
+        _check(x.to(cuda)[:, offset:], tokens, k)
+
+
 def test_row_splits_give_one_answer(cuda):
     """A row's ids and rank do not depend on how many rows are scored with it, its sums only in rounding."""
     from nebulasd_b200.logprobs import token_logprobs
@@ -237,6 +262,51 @@ def test_streams_and_graphs(cuda):
             assert all(torch.equal(a, b) for a, b in zip(out, token_logprobs(logits, tokens, 4)))
 
 
+def test_two_calls_at_once(cuda):
+    """Calls on two streams share nothing but the error word."""
+    from nebulasd_b200.logprobs import token_logprobs, workspace_errors
+    sets = [_logits(60 + i, rows, vocab, dtype, cuda)
+            for i, (rows, vocab, dtype) in enumerate([(5, 151936, torch.float16), (300, 9001, torch.float32)])]
+    want = [token_logprobs(x, t, 20) for x, t in sets]
+    torch.cuda.synchronize()
+    workspace_errors()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[] for _ in sets]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(token_logprobs(*sets[i], 20))
+    torch.cuda.synchronize()
+    for one, all_of in zip(want, got):
+        assert all(torch.equal(a, b) for g in all_of for a, b in zip(g, one))
+    assert workspace_errors() == 0
+
+
+@pytest.mark.parametrize("dtype,rows", [(torch.bfloat16, 460), (torch.float16, 80)])
+def test_whole_vocabulary_batches(dtype, rows, cuda):
+    """More rows than the GPU holds at once, and a verify batch, against 64-bit torch on the GPU."""
+    from nebulasd_b200.logprobs import token_logprobs
+    vocab = 151936
+    g = torch.Generator(device=cuda).manual_seed(rows)
+    logits = (torch.randn((rows, vocab), generator=g, device=cuda) * 3).to(dtype)
+    tokens = torch.randint(0, vocab, (rows,), generator=g, device=cuda).to(torch.int32)
+    tokens[::2] = logits.argmax(1)[::2].to(torch.int32)
+    tokens[5] = -1
+    got = token_logprobs(logits, tokens, 32)
+    for r in range(0, rows, 20):
+        x, t = logits[r:r + 20].double(), tokens[r:r + 20].long()
+        logp = torch.log_softmax(x, 1)
+        ids = torch.sort(x, dim=1, descending=True, stable=True).indices[:, :32]
+        assert torch.equal(got.top_ids[r:r + 20].long(), ids)
+        _close(got.top_logprobs[r:r + 20], logp.gather(1, ids).cpu(), vocab)
+        _close(got.entropy[r:r + 20], -(logp.exp() * logp).sum(1).cpu(), vocab)
+        own = t.clamp(min=0)[:, None]
+        given = torch.where(t >= 0, logp.gather(1, own)[:, 0], math.nan)
+        _close(got.logprobs[r:r + 20], given.cpu(), vocab)
+        ranks = torch.where(t >= 0, 1 + (x > x.gather(1, own)).sum(1), 0)
+        assert torch.equal(got.ranks[r:r + 20].long(), ranks)
+
+
 def test_empty_batch(cuda):
     from nebulasd_b200.logprobs import token_logprobs
     got = token_logprobs(torch.empty((0, 100), dtype=torch.float16, device=cuda),
@@ -252,3 +322,6 @@ def test_refusals_on_the_device(cuda):
                  (x[:, :5], None, 6), (x, None, -1), (x.double(), None, 0), (x[:, :0], None, 0)):
         with pytest.raises(ValueError):
             token_logprobs(*args)
+    for shape in ((1 << 31, 1), (1, (1 << 30) + 1)):  # (one element in memory)
+        with pytest.raises(ValueError):
+            token_logprobs(x[:1, :1].as_strided(shape, (0, 1) if shape[1] == 1 else (1 << 30, 0)))

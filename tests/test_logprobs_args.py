@@ -33,6 +33,11 @@ def test_the_c_entry_refuses(kw):
     assert _lib.lib.neb_last_error()
 
 
+def test_rows_beyond_an_int_are_refused():
+    assert _call(vocab=1 << 30) == OK
+    assert _call(vocab=(1 << 30) + 1) == _lib.NEB_ERR_UNSUPPORTED
+
+
 def test_host_tensors_are_refused():
     with pytest.raises(ValueError):
         token_logprobs(torch.zeros((2, 10), dtype=torch.float16))
