@@ -36,12 +36,14 @@ def _check_caches(k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, in
     token_bytes = dim * k_cache.element_size()
     if k_cache.numel() == 0 or token_bytes % 16:
         raise ValueError("the caches must hold blocks whose head rows are a multiple of 16 bytes")
+    if layers * heads * size * token_bytes >= 1 << 31 or nb >= 1 << 31:
+        raise ValueError("the caches must hold fewer than 2^31 blocks of less than 2 GiB")
     return nb, layers * heads, size, token_bytes
 
 
 def _check_list(name: str, t: torch.Tensor, index: int, length: int | None = None) -> None:
     if (t.dtype != torch.int32 or t.dim() != 1 or t.get_device() != index or not t.is_contiguous()
-            or (length is not None and t.shape[0] != length)):
+            or t.shape[0] >= 1 << 31 or (length is not None and t.shape[0] != length)):
         raise ValueError(f"{name} must be a contiguous int32 vector on the caches' device"
                          + (f" of {length} elements" if length is not None else ""))
 
@@ -111,8 +113,9 @@ class BlockPool:
         shape = _check_caches(k_cache, v_cache)
         index = k_cache.get_device()
         if (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.get_device() != index
-                or not block_table.is_contiguous() or block_table.numel() == 0):
-            raise ValueError("block_table must be a contiguous int32 [rows, max_blocks] tensor on the caches' device")
+                or not block_table.is_contiguous() or not 0 < block_table.numel() < 1 << 31):
+            raise ValueError("block_table must be a contiguous int32 [rows, max_blocks] tensor on the caches' "
+                             "device, of fewer than 2^31 entries")
         _check_list("seq_blocks", seq_blocks, index, block_table.shape[0])
         _check_list("ref_counts", ref_counts, index, shape[0])
         self.k_cache, self.v_cache = k_cache, v_cache

@@ -297,6 +297,35 @@ def test_captured_round(cuda):
         same(h, pool)
 
 
+def test_two_pools_at_once(cuda):
+    """Rounds on two pools, each on its own stream."""
+    pools, handles, lists = [], [], []
+    for seed in (31, 32):
+        pool, groups, empty = make_pool(seed, num_blocks=3000, rows=40, width=80, lens=[900, 1200, 33, 640], fan=2, layers=3,
+                                        heads=2)
+        pools.append(pool)
+        handles.append(to_device(pool, cuda))
+        live = [r for g in groups for r in g]
+        lists.append((live, empty[:8], [900, 900, 1195, 1200, 33, 31, 640, 500], live[::2]))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in pools]
+    args = [[ints(x, cuda) for x in some] for some in lists]
+    torch.cuda.synchronize()
+    for h, (parents, children, lens, drop), s in zip(handles, args, streams):
+        with torch.cuda.stream(s):
+            h.fork(parents, children, lens)
+            h.free(drop)
+            h.compact()
+            h.fork(children, parents, lens)  # the dropped rows take them, the others refuse
+    torch.cuda.synchronize()
+    for pool, h, (parents, children, lens, drop) in zip(pools, handles, lists):
+        bits = oracle.fork(pool, parents, children, lens) | oracle.free(pool, drop)
+        bits |= oracle.compact(pool)[0]
+        bits |= oracle.fork(pool, children, parents, lens)
+        assert bits == h.errors() == oracle.INVALID
+        same(h, pool)
+
+
 def test_another_stream(cuda):
     pool, groups, empty = make_pool(22, num_blocks=100, rows=12, width=12, lens=[100, 70], layers=2, heads=1)
     h = to_device(pool, cuda)
