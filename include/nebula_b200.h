@@ -201,7 +201,8 @@ int neb_greedy_accept(const void* logits, int64_t row_stride, int32_t vocab, int
  * nebulasd_b200.logprobs.token_logprobs.
  *
  * logits        [num_rows][row_stride] of `dtype` (NEB_DTYPE_*), the first
- *               `vocab` of each row used; rows may start at any element
+ *               `vocab` (up to 2^30) of each row used; rows may start at any
+ *               element
  * token_ids     [num_rows] or NULL: the row's given token t, or -1 for none
  * logprobs      [num_rows]: x_t - log(sum_j exp(x_j)); NaN without a token
  * ranks         [num_rows]: 1 + the number of logits larger than x_t; 0
