@@ -345,7 +345,9 @@ int neb_copy_blocks(void* k_cache, void* v_cache, int64_t num_blocks, int32_t ti
  * child whose turn comes after the free blocks are spent is refused (bit 8).
  * Refused as well: a row that is not empty, or listed again after its first
  * time, a length beyond the parent's blocks (bit 4).  A refused child's row
- * stays empty.  An entry of the parent out of range is copied as -1 (bit 0).
+ * stays empty.  An entry of the parent out of range is copied as -1 (bit 0); a
+ * block of the parent that had no positive count before the call is shared all
+ * the same, but its tokens are not copied (bit 7).
  * Workspace: neb_fork_workspace_bytes, 16-byte aligned, any contents. */
 size_t neb_fork_workspace_bytes(int64_t num_blocks, int32_t num_children);
 int neb_fork_sequences(void* k_cache, void* v_cache, int64_t num_blocks, int32_t tiles_per_block,

@@ -185,9 +185,11 @@ __device__ __forceinline__ void cluster_share(int* slots, int value) {
   }
 }
 
-// Bits of the part's blocks whose count satisfies `bit`; returns how many (over the CTA).
-template <typename Bit>
-__device__ __forceinline__ int build_map(PlanShared& sh, const PlanPart& part, const int32_t* refs, Bit bit) {
+// Bits of the part's blocks whose count satisfies `bit`; returns how many (over the CTA).  The warp that has a word
+// calls also(word, in, count) for its blocks.
+template <typename Bit, typename Also>
+__device__ __forceinline__ int build_map(PlanShared& sh, const PlanPart& part, const int32_t* refs, Bit bit,
+                                         Also also) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int kAhead = 16;  // words of a warp whose counts are loaded before the first is used
   int mine = 0;
@@ -202,7 +204,9 @@ __device__ __forceinline__ int build_map(PlanShared& sh, const PlanPart& part, c
     for (int u = 0; u < kAhead; ++u) {
       const int at = w + u * kPlanWarps;
       if (at >= part.words) break;
-      const unsigned int word = __ballot_sync(~0u, 32 * at + lane < part.count && bit(r[u]));
+      const bool in = 32 * at + lane < part.count;
+      const unsigned int word = __ballot_sync(~0u, in && bit(r[u]));
+      also(at, in, r[u]);
       if (lane == 0) sh.map[at] = word;
       mine += __popc(word);
     }
@@ -234,10 +238,13 @@ struct ForkParams {
   const int32_t* lens;
   const int32_t* capacities;  // or null
   int n;
-  int32_t* plan;   // [n][4]: shared blocks, all blocks (-1: refused), first of its slots, partial tokens
-  int32_t* slots;  // free blocks, lowest first
+  int32_t* plan;     // [n][4]: shared blocks, all blocks (-1: refused), first of its slots, partial tokens
+  int32_t* partial;  // [n]: the partial tokens' block, or kNoBlock, kNoCount
+  int32_t* slots;    // free blocks, lowest first
+  unsigned int* uncounted;  // a bit per block: no positive count before the call
   unsigned int* error_bits;
 };
+constexpr int kNoBlock = -1, kNoCount = -2;  // an index out of range; a block without a positive count
 
 // The children's shapes and their slots in order, by the first CTA, a child per thread and round: three round
 // trips to memory for up to 1,024 children.  Returns the slots needed; `last` is the thread's child of the last
@@ -256,12 +263,17 @@ __device__ __forceinline__ int plan_children(const ForkParams& p, int* sums, int
     const int shared = max(len, 0) / bs;
     const int total = (int)(((long long)max(max(len, room), 0) + bs - 1) / bs);
     if (total > p.t.width) bad |= kErrTooManyBlocks;
+    const int part = max(len, 0) - shared * bs;
+    int from = kNoBlock, count = 1;  // the partial tokens' block, its count
     if (in && !bad) {
       // Both rows as they were before the round's claims.  (A claim of an earlier round is negative: its row is
       // neither empty nor long enough for a parent, as it would be refused within one round.)
       const int held = __ldcg(&p.t.seq_blocks[child]), of_parent = len > 0 ? __ldcg(&p.t.seq_blocks[parent]) : 0;
+      if (part > 0) from = p.t.table[(long long)parent * p.t.width + shared];  // (shared < total <= width)
       if (held != 0 || (len > 0 && ((long long)len + bs - 1) / bs > of_parent)) bad |= kErrInvalidRows;
     }
+    if (from < 0 || from >= p.c.num_blocks) from = kNoBlock;
+    else count = p.t.refs[from];
     __syncthreads();
     // A row listed twice goes to its first child: the lowest claim wins.
     if (in && !bad) atomicMin(&p.t.seq_blocks[child], i - p.n);
@@ -270,8 +282,11 @@ __device__ __forceinline__ int plan_children(const ForkParams& p, int* sums, int
     if (in && bad) report(p.error_bits, bad);
     int all;
     const int before = block_scan(in && !bad ? total - shared : 0, sums, all);
-    last = make_int4(shared, bad ? -1 : total, need + before, max(len, 0) - shared * bs);
-    if (in) reinterpret_cast<int4*>(p.plan)[i] = last;
+    last = make_int4(shared, bad ? -1 : total, need + before, part);
+    if (in) {
+      reinterpret_cast<int4*>(p.plan)[i] = last;
+      p.partial[i] = count > 0 ? from : kNoCount;
+    }
     need += all;
   }
   return need;
@@ -291,7 +306,12 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const __grid_co
     need = plan_children(p, sh.sums, last);
   } else {
     part = plan_part(p.c.num_blocks, blockIdx.x - 1, kMapCtas);
-    is_free = build_map(sh, part, p.t.refs, [](int r) { return r == 0; });
+    is_free = build_map(
+        sh, part, p.t.refs, [](int r) { return r == 0; },
+        [&](int at, bool in, int r) {
+          const unsigned int word = __ballot_sync(~0u, in && r <= 0);
+          if ((threadIdx.x & 31) == 0) p.uncounted[part.first / 32 + at] = word;
+        });
   }
   asm volatile("barrier.cluster.wait;" ::: "memory");  // every CTA has started
   cluster_share(sh.cta_bits, is_free);
@@ -345,28 +365,31 @@ __global__ void __launch_bounds__(kCopyThreads, kPartCtas) fork_kernel(const __g
       const int j = j0 + lane + 32 * u;
       b[u] = j < shared ? from[j] : j < total ? fresh[j] : -1;
     }
+    // Whether a shared block had a count is looked up as it was before the call: in a broken pool it may be one of
+    // the fresh blocks too, and its count then rises by one for each row in either order.
+    unsigned int lack[kEntries / 32];
+#pragma unroll
+    for (int u = 0; u < kEntries / 32; ++u)
+      lack[u] = j0 + lane + 32 * u < shared && b[u] >= 0 && b[u] < p.c.num_blocks ? p.uncounted[b[u] >> 5] : 0u;
 #pragma unroll
     for (int u = 0; u < kEntries / 32; ++u) {
       const int j = j0 + lane + 32 * u;
       if (j >= total) break;
-      if (j < shared) {
-        if (b[u] < 0 || b[u] >= p.c.num_blocks) {
-          report(p.error_bits, kErrBlockIndex);
-          b[u] = -1;
-        } else if (atomicAdd(&p.t.refs[b[u]], 1) <= 0) {
-          report(p.error_bits, kErrRefCount);
-        }
+      if (b[u] < 0 || b[u] >= p.c.num_blocks) {  // (of a shared one)
+        report(p.error_bits, kErrBlockIndex);
+        b[u] = -1;
       } else {
-        p.t.refs[b[u]] = 1;
+        atomicAdd(&p.t.refs[b[u]], 1);
+        if ((lack[u] >> (b[u] & 31)) & 1) report(p.error_bits, kErrRefCount);
       }
       to[j] = b[u];
     }
   }
-  // The partial blocks.  A pair takes three loads that depend on each other: once per CTA for the first children.
+  // The partial blocks.  A pair takes two loads that depend on each other: once per CTA for the first children.
   auto look_up = [&](int i) {
     const int4 plan = reinterpret_cast<const int4*>(p.plan)[i];
     if (plan.y < 0 || plan.w == 0) return Pair{-1, -1, 0};
-    return Pair{p.t.table[(long long)p.parents[i] * p.t.width + plan.x], p.slots[plan.z], plan.w};
+    return Pair{p.partial[i], p.slots[plan.z], plan.w};
   };
   __shared__ Pair known[kCopyThreads];
   if ((int)threadIdx.x < p.n) known[threadIdx.x] = look_up(threadIdx.x);
@@ -375,8 +398,8 @@ __global__ void __launch_bounds__(kCopyThreads, kPartCtas) fork_kernel(const __g
       p.c, p.n, [&](int i) { return i < kCopyThreads ? known[i] : look_up(i); },
       [&](int, const Pair& a) {
         if (a.tokens == 0) return false;
-        if (a.src >= 0 && a.src < p.c.num_blocks) return true;
-        if (threadIdx.x == 0) report(p.error_bits, kErrBlockIndex);
+        if (a.src >= 0) return true;
+        if (threadIdx.x == 0) report(p.error_bits, a.src == kNoCount ? kErrRefCount : kErrBlockIndex);
         return false;
       });
 }
@@ -455,7 +478,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const __grid
   pdl_trigger();
   const PlanPart part = plan_part(p.c.num_blocks, blockIdx.x, kPlanCtas);
   asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
-  const int used = build_map(sh, part, p.t.refs, [](int r) { return r > 0; });
+  const int used = build_map(sh, part, p.t.refs, [](int r) { return r > 0; }, [](int, bool, int) {});
   asm volatile("barrier.cluster.wait;" ::: "memory");  // every CTA has started
   cluster_share(sh.cta_bits, used);
   cluster_sync();
@@ -656,7 +679,7 @@ int neb_copy_blocks(void* k_cache, void* v_cache, int64_t num_blocks, int32_t ti
 
 size_t neb_fork_workspace_bytes(int64_t num_blocks, int32_t num_children) {
   if (num_blocks <= 0 || num_blocks > INT_MAX || num_children < 0) return 0;
-  return 16 * (size_t)num_children + 4 * (size_t)num_blocks;
+  return 20 * (size_t)num_children + 4 * (size_t)num_blocks + 4 * (((size_t)num_blocks + 31) / 32);
 }
 
 int neb_fork_sequences(void* k_cache, void* v_cache, int64_t num_blocks, int32_t tiles_per_block, int32_t block_size,
@@ -682,7 +705,9 @@ int neb_fork_sequences(void* k_cache, void* v_cache, int64_t num_blocks, int32_t
   p.capacities = capacities;
   p.n = num_children;
   p.plan = static_cast<int32_t*>(workspace);
-  p.slots = p.plan + 4ll * num_children;
+  p.partial = p.plan + 4ll * num_children;
+  p.slots = p.partial + num_children;
+  p.uncounted = reinterpret_cast<unsigned int*>(p.slots + num_blocks);
   p.error_bits = error_bits;
   unsigned grid = 1;
   const long long rows = (long long)num_children * (p.t.width / kEntries + 1);

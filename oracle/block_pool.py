@@ -80,18 +80,20 @@ def fork(p: Pool, parents, children, lens, capacities=None) -> int:
                 bits |= BLOCK
                 b = -1
             else:
-                if p.refs[b] <= 0:
+                if start.refs[b] <= 0:
                     bits |= REFS
                 p.refs[b] += 1
             p.table[ch, j] = b
         for j in range(need):
             b = free[first + j]
-            p.refs[b] = 1
+            p.refs[b] += 1
             p.table[ch, shared + j] = b
         p.held[ch] = total
         if n % size:
             s, d = int(start.table[par, shared]), free[first]
-            if 0 <= s < nb:
+            if 0 <= s < nb and start.refs[s] <= 0:
+                bits |= REFS
+            elif 0 <= s < nb:
                 p.k[d, :, :, :n % size], p.v[d, :, :, :n % size] = (start.k[s, :, :, :n % size],
                                                                     start.v[s, :, :, :n % size])
             else:

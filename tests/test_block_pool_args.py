@@ -115,3 +115,20 @@ def test_oracle_known_answers():
     assert oracle.fork(pool, [a], [c], [49], None) == oracle.INVALID
     assert oracle.fork(pool, [a], [c], [0], [65]) == oracle.WIDTH
     assert oracle.fork(pool, [a, a], [c, c], [16, 16], None) == oracle.INVALID and pool.held[c] == 1
+
+
+def test_oracle_counts_every_row_of_a_broken_pool():
+    """A block in use that is counted as free is shared, given out as a fresh one too, and reported."""
+    pool, groups, empty = make_pool(2, num_blocks=6, rows=4, width=4, lens=[40], layers=1, heads=1, dim=8)
+    a, lost = groups[0][0], int(pool.table[groups[0][0], 1])
+    pool.refs[lost] = 0
+    for order in ([0, 1], [1, 0]):
+        now, (c, d) = pool.copy(), empty[:2]
+        lens, caps = np.array([32, 0])[order], np.array([32, 64])[order]  # takes all four free blocks
+        assert oracle.fork(now, [a, a], [c, d], lens, caps) == oracle.REFS
+        assert now.refs[lost] == 2 == sum(int((now.table[r] == lost).sum()) for r in (c, d))
+    pool.refs[lost], last = 1, pool.table[a, 2]
+    pool.refs[last] = 0
+    now = pool.copy()
+    assert oracle.fork(now, [a], [empty[0]], [40]) == oracle.REFS
+    assert np.array_equal(now.k, pool.k)  # nothing copied from a block that may be given out

@@ -132,6 +132,28 @@ def test_fork_reports_broken_tables(cuda):
     _fork(h, pool, [a, b], empty[:2], [64, 70], None, cuda)
 
 
+def test_fork_from_blocks_without_a_count(cuda):
+    """Blocks in use that are counted as free (or less), handed out as fresh ones by the same call: shared, counted
+    and reported whatever comes first, and not copied from."""
+    broken, groups, empty = make_pool(14, num_blocks=40, rows=24, width=9, lens=[100, 100, 100], layers=3, heads=2)
+    a, b, c = (g[0] for g in groups)
+    broken.refs[broken.table[a, [2, 6]]] = 0   # 100 tokens: six full blocks and four tokens
+    broken.refs[broken.table[b, [0, 6]]] = -2, -1
+    parents, lens = [a, b, c, a, a, b, c, a, 0, 0], [100, 100, 100, 50, 100, 97, 16, 99, 0, 0]
+    caps = [128, 128, 101, 80, 128, 97, 80, 144, 32, 32]
+    for turn in range(30):
+        pool, h = broken.copy(), to_device(broken, cuda)
+        _fork(h, pool, parents, empty[:10], lens, caps, cuda)
+        # all free blocks are spent: one counted zero is left, the -2 that two rows have raised
+        assert int((pool.refs == 0).sum()) == 1 and pool.refs[pool.table[a, 2]] == 4 + 1
+    # each alone: a shared block, a partial one
+    for row, n in ((a, 48), (a, 99), (b, 16), (b, 97)):
+        pool, h = broken.copy(), to_device(broken, cuda)
+        h.fork(ints([row], cuda), ints(empty[:1], cuda), ints([n], cuda))
+        assert oracle.fork(pool, [row], empty[:1], [n]) == h.errors() == oracle.REFS
+        same(h, pool)
+
+
 @pytest.mark.parametrize("n,num_blocks", [(300, 20000), (1500, 135168), (64, 1000003)])
 def test_fork_many(n, num_blocks, cuda):
     rng = np.random.default_rng(n)
