@@ -617,9 +617,9 @@ __device__ __forceinline__ Part join(const Part* parts, int n) {
 }
 
 // Any row, logit by logit, by one CTA: rows with a NaN or +inf (results NaN, order over all values) and rows
-// that have nothing above kLow.  Slow, as such rows are rare: a wholly masked row of 151,936 fp16 logits 44 us, with
-// 20 alternatives 103 us (their largest in one pass of keys; a pass per alternative took 619 us), beside the 12 us
-// and 20 us of a call for another row.
+// that have nothing above kLow.  Slow, as such rows are rare: 151,936 fp16 logits at the lowest value 42 us, with
+// 20 alternatives 100 us (their largest in one pass of keys; a pass per alternative took 619 us), beside the 6 us
+// and 12 us of another row (device times in a graph).
 template <typename T>
 __device__ __noinline__ void general_row(Shared& sh, const Params& p, const void* x, int row, int head, int tok) {
   const int tid = threadIdx.x;
@@ -656,11 +656,24 @@ __device__ __noinline__ void general_row(Shared& sh, const Params& p, const void
     s += sh.warp_f[1][i];
     w += sh.warp_f[2][i];
   }
-  const float ln_s = s > 0.f ? logf(s) : nan;
+  float r = s - 1.f;
+  if (s < 2.f) {  // a confident row: summed again without its maximum
+    r = 0.f;
+    for (int j = tid; j < p.vocab; j += kThreads) {
+      const float v = Elem<T>::load(x, j);
+      r += v == m ? 0.f : fast_exp2((v - m) * kLog2e);
+    }
+    r = warp_sum(r);
+    if ((tid & 31) == 0) sh.warp_f[3][tid >> 5] = r;
+    __syncthreads();
+    r = 0.f;
+    for (int i = 0; i < kWarps; ++i) r += sh.warp_f[3][i];
+  }
+  const float ln_s = log1pf(r);
   if (tid == 0) {
     if (p.logprobs) p.logprobs[row] = tok >= 0 ? (Elem<T>::load(x, tok) - m) - ln_s : nan;
     if (p.ranks) p.ranks[row] = tok >= 0 ? 1 + above : 0;
-    if (p.entropy) p.entropy[row] = ln_s - kLn2 * (w / s);
+    if (p.entropy) p.entropy[row] = ln_s - kLn2 * (w / (1.f + r));
   }
   const int k = p.num_top;
   if (k == 0) return;

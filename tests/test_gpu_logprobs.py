@@ -152,6 +152,27 @@ def test_confident_rows_keep_their_precision(dtype, rows, cuda):
     assert got.ranks.tolist() == rk.tolist() and got.top_ids.tolist() == ids.tolist()
 
 
+@pytest.mark.parametrize("dtype,top,rest", [(torch.float16, -65024.0, -65056.0), (torch.float32, 70000.0, 69980.0),
+                                            (torch.float32, -70000.0, -70024.0), (torch.float32, 1e6, 1e6 - 15.0)])
+@pytest.mark.parametrize("rows", [1, 500])
+def test_confident_rows_far_from_zero_keep_their_precision(dtype, top, rest, rows, cuda):
+    """The same where the logits are too far from 0 for the one-pass sums."""
+    from nebulasd_b200.logprobs import token_logprobs
+    vocab = 20000
+    _, tokens = _logits(rows, rows, vocab, dtype, cuda)
+    logits = torch.full((rows, vocab), rest, dtype=dtype, device=cuda)
+    logits[:, ::5] = -math.inf
+    logits[torch.arange(rows), tokens.long()] = top
+    logits[0, ::2] = top  # (one with many at the maximum)
+    got = token_logprobs(logits, tokens, 2)
+    lp, rk, ent, ids, tops = oracle(logits, tokens.tolist(), 2)
+    g = (-(-vocab // 128) + 64) * 2.0 ** -24
+    for a, b in ((got.logprobs, lp), (got.entropy, ent), (got.top_logprobs, tops)):
+        a, b = a.double().cpu(), torch.as_tensor(b)
+        assert bool(((a - b).abs() <= 4 * g * b.abs()).all())
+    assert got.ranks.tolist() == rk.tolist() and got.top_ids.tolist() == ids.tolist()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows", [1, 30, 500])
 def test_fewer_allowed_tokens_than_alternatives(dtype, rows, cuda):
