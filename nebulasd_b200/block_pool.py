@@ -43,7 +43,7 @@ def _check_caches(k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, in
 
 def _check_list(name: str, t: torch.Tensor, index: int, length: int | None = None) -> None:
     if (t.dtype != torch.int32 or t.dim() != 1 or t.get_device() != index or not t.is_contiguous()
-            or t.shape[0] >= 1 << 31 or (length is not None and t.shape[0] != length)):
+            or t.numel() >= 1 << 31 or (length is not None and t.numel() != length)):
         raise ValueError(f"{name} must be a contiguous int32 vector on the caches' device"
                          + (f" of {length} elements" if length is not None else ""))
 
@@ -61,7 +61,7 @@ def copy_blocks(k_cache: torch.Tensor, v_cache: torch.Tensor, src: torch.Tensor,
     must come before any graph capture.
     """
     nb, tiles, size, token_bytes = _check_caches(k_cache, v_cache)
-    index, n = k_cache.get_device(), src.shape[0] if src.dim() else 0
+    index, n = k_cache.get_device(), src.numel()
     _check_list("src", src, index)
     _check_list("dst", dst, index, n)
     if num_tokens is not None:
@@ -105,7 +105,8 @@ class BlockPool:
     ``ref_counts`` int32 ``[num_blocks]``: how many rows use each block.  All
     contiguous, on the caches' device.  Methods run on the current stream of
     that device, and calls on one pool must be ordered.  What they refuse they
-    leave as it was; ``errors`` tells why.
+    leave as it was; ``errors`` tells why.  The tensors stay where they were when
+    the pool was made: with one replaced or moved, every method raises.
     """
 
     def __init__(self, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -124,10 +125,16 @@ class BlockPool:
         self._index, self._device = index, k_cache.device
         self._caches = (k_cache.data_ptr(), v_cache.data_ptr(), *shape)
         self._tables = (block_table.data_ptr(), *block_table.shape, seq_blocks.data_ptr(), ref_counts.data_ptr())
+        self._places = (*self._caches[:2], self._tables[0], *self._tables[3:])
         self._fork_bytes: dict[int, int] = {}
         self._compact_bytes = _lib.lib.neb_compact_workspace_bytes(shape[0])
         self._word = new_error_word(index, "BlockPool")
         self._error_ptr = self._word.data_ptr()
+
+    def _check_tensors(self) -> None:
+        if (self.k_cache.data_ptr(), self.v_cache.data_ptr(), self.block_table.data_ptr(), self.seq_blocks.data_ptr(),
+                self.ref_counts.data_ptr()) != self._places:
+            raise ValueError("a tensor of the pool has been replaced or moved since the pool was made")
 
     def _temporary(self, need: int) -> torch.Tensor:
         # From the caching allocator, so that calls on several streams and captured
@@ -145,7 +152,8 @@ class BlockPool:
         is not empty or is listed before, a length beyond the parent's blocks (bit 4), rows out of range (bit
         1), more than ``max_blocks`` blocks (bit 2), too few free blocks (bit 8).  Int32 vectors.
         """
-        index, n = self._index, children.shape[0] if children.dim() else 0
+        self._check_tensors()
+        index, n = self._index, children.numel()
         _check_list("children", children, index)
         _check_list("parents", parents, index, n)
         _check_list("seq_lens", seq_lens, index, n)
@@ -164,9 +172,10 @@ class BlockPool:
     def free(self, rows: torch.Tensor) -> None:
         """Empty the listed rows (int32): their blocks lose one reference each and are free at 0.  A row
         listed twice is freed once."""
+        self._check_tensors()
         _check_list("rows", rows, self._index)
         with _Device(self._index):
-            rc = _lib.lib.neb_free_sequences(*self._tables, self.num_blocks, rows.data_ptr(), rows.shape[0],
+            rc = _lib.lib.neb_free_sequences(*self._tables, self.num_blocks, rows.data_ptr(), rows.numel(),
                                              self._error_ptr, _raw_stream(self._index))
         _lib.check(rc, "free")
 
@@ -175,6 +184,7 @@ class BlockPool:
 
         Contents, counts and every row's entries move along.  Returns int32 ``[num_blocks]``: each block's
         new index (-1: it was free), for ids that the caller keeps elsewhere."""
+        self._check_tensors()
         need = self._compact_bytes
         with _Device(self._index):
             ws = self._temporary(need)

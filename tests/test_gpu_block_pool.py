@@ -277,6 +277,26 @@ def test_refusals_on_the_device(cuda):
     same(h, pool)
 
 
+@pytest.mark.parametrize("name", ["k_cache", "v_cache", "block_table", "seq_blocks", "ref_counts"])
+def test_replaced_tensors_are_refused(name, cuda):
+    """A pool whose tensor has other memory, or another tensor, neither reads nor writes where it was."""
+    pool, groups, empty = make_pool(23, num_blocks=12, rows=4, width=4, lens=[40], layers=1, heads=1)
+    h = to_device(pool, cuda)
+    child, n = ints(empty[:1], cuda), ints([40], cuda)
+    t, old = getattr(h, name), getattr(h, name).data
+    other = old.clone()
+    calls = (lambda: h.fork(ints(groups[0], cuda), child, n), lambda: h.free(child), h.compact)
+    for put, back in ((lambda: setattr(t, "data", other), lambda: setattr(t, "data", old)),
+                      (lambda: setattr(h, name, other), lambda: setattr(h, name, t))):
+        put()
+        for call in calls:
+            with pytest.raises(ValueError, match="replaced"):
+                call()
+        back()
+        same(h, pool)
+    _fork(h, pool, groups[0], empty[:1], [40], None, cuda)
+
+
 def test_captured_round(cuda):
     """Fork, copy, free and compact captured twice (two graphs of one pool), replayed with new lists in place."""
     from nebulasd_b200.block_pool import copy_blocks, workspace_errors
