@@ -162,6 +162,12 @@ int neb_paged_attention_verify_long(const void* q, const void* k_cache, const vo
  * so call it before reusing a workspace whose last call may have failed. */
 int neb_workspace_status(void* workspace, uint32_t* error_bits, void* stream);
 
+/* For the entries that take an error_bits word of their own (log probabilities,
+ * block pool): moves its bits to *taken and clears it, in one step, so that no bit
+ * is lost that a call on another stream records meanwhile.  Both are device
+ * memory; does not synchronise. */
+int neb_take_error_bits(uint32_t* error_bits, uint32_t* taken, void* stream);
+
 /* ---------------------------------------------------------------- greedy accept
  * Greedy speculative acceptance on the device.  Replaces the verify-side tail
  * of the reference: torch.argmax of the logits

@@ -48,6 +48,7 @@ SIGNATURES = {
     "neb_greedy_accept_workspace_bytes": ([_i32], _sz),
     "neb_greedy_accept": ([_vp, _i64, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp,
                            _sz, _vp], ctypes.c_int),
+    "neb_take_error_bits": ([_vp, _vp, _vp], ctypes.c_int),
     "neb_token_logprobs": ([_vp, _i32, _i64, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
                            ctypes.c_int),
     "neb_copy_blocks": ([_vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _i32, _vp, _vp], ctypes.c_int),

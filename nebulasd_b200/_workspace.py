@@ -115,7 +115,9 @@ def new_error_word(index: int, what: str) -> torch.Tensor:
 
 
 def read_error_word(t: torch.Tensor) -> int:
-    bits = int(t.item()) & 0xFFFFFFFF
-    if bits:
-        t.zero_()
-    return bits
+    """Synchronise the current stream of the word's device; return and clear the bits, in one step on the device."""
+    with torch.cuda.device(t.device):
+        taken = torch.empty_like(t)
+        rc = _lib.lib.neb_take_error_bits(t.data_ptr(), taken.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        _lib.check(rc, "neb_take_error_bits")
+        return int(taken.item()) & 0xFFFFFFFF

@@ -197,5 +197,4 @@ class BlockPool:
     def errors(self) -> int:
         """Synchronise the current stream; return and clear the error bits that the pool's calls recorded
         (the bits of ``neb_fork_sequences`` and its neighbours in the C header)."""
-        with _Device(self._index):
-            return read_error_word(self._word)
+        return read_error_word(self._word)

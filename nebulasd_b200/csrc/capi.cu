@@ -269,6 +269,18 @@ extern "C" int neb_workspace_status(void* workspace, uint32_t* error_bits, void*
   return read_and_clear_status(workspace, error_bits, static_cast<cudaStream_t>(stream));
 }
 
+namespace neb {
+// One step, so that a bit that another stream records meanwhile is either in *taken or still in *error_bits.
+static __global__ void take_error_bits_kernel(uint32_t* error_bits, uint32_t* taken) { *taken = atomicExch(error_bits, 0u); }
+}  // namespace neb
+
+extern "C" int neb_take_error_bits(uint32_t* error_bits, uint32_t* taken, void* stream) {
+  NEB_REQUIRE(error_bits && taken, NEB_ERR_INVALID, "null argument");
+  take_error_bits_kernel<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(error_bits, taken);
+  NEB_CUDA(cudaGetLastError());
+  return NEB_OK;
+}
+
 // ------------------------------------------------- allocation-free decode attention
 // For callers that cannot allocate device memory: the split-K scratch of the
 // decode kernel lives in one statically sized __device__ array of this

@@ -132,3 +132,8 @@ def test_oracle_counts_every_row_of_a_broken_pool():
     now = pool.copy()
     assert oracle.fork(now, [a], [empty[0]], [40]) == oracle.REFS
     assert np.array_equal(now.k, pool.k)  # nothing copied from a block that may be given out
+
+
+def test_error_words_that_are_missing():
+    _refused(L.neb_take_error_bits(None, A, None))
+    _refused(L.neb_take_error_bits(A, None, None))

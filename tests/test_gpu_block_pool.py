@@ -73,6 +73,30 @@ def test_copy_far_blocks(cuda):
     assert int((k[2:19998] != 0).sum()) == 0
 
 
+def test_error_bits_of_another_stream_are_kept(cuda):
+    """Bits are read while a call on another stream records its own: every read takes some, none is lost."""
+    from nebulasd_b200.block_pool import copy_blocks, workspace_errors
+    pool, _, _ = make_pool(24, num_blocks=8, rows=1, width=1, lens=[], layers=1, heads=1)
+    h = to_device(pool, cuda)
+    bad, clash = (ints([0, 1], cuda), ints([4, 9], cuda)), (ints([2, 3], cuda), ints([6, 6], cuda))
+    want = pool.copy()
+    assert oracle.copy_blocks(want.k, want.v, [0, 1], [4, 9]) | oracle.copy_blocks(want.k, want.v, [2, 3], [6, 6]) \
+        == oracle.BLOCK | oracle.CONFLICT
+    workspace_errors()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for turn in range(300):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(1500 * (turn % 50))  # up to some 40 us
+            copy_blocks(h.k_cache, h.v_cache, *clash)
+        copy_blocks(h.k_cache, h.v_cache, *bad)
+        bits = workspace_errors()
+        assert bits & oracle.BLOCK
+        side.synchronize()
+        assert bits | workspace_errors() == oracle.BLOCK | oracle.CONFLICT
+    same(h, want)
+
+
 # ------------------------------------------------------------------------ fork
 def _fork(h, pool, parents, children, lens, caps, dev):
     h.fork(ints(parents, dev), ints(children, dev), ints(lens, dev), None if caps is None else ints(caps, dev))
