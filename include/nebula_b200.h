@@ -221,7 +221,8 @@ int neb_greedy_accept(const void* logits, int64_t row_stride, int32_t vocab, int
  * +inf, or nothing but -inf, gets NaN for every floating result; its order is
  * still defined (a NaN counts as the largest value, -0 equals +0).  A token
  * outside [-1, vocab) is treated as -1 and recorded as bit 6 of *error_bits
- * (device memory, optional; bit 3: a bounded wait gave up, the row is wrong).
+ * (device memory, optional; bit 3: a bounded wait gave up, and the row was read
+ * again, slowly).
  * Needs no workspace, keeps nothing between calls. */
 #define NEB_DTYPE_F16 0
 #define NEB_DTYPE_BF16 1

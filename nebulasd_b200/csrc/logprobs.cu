@@ -616,10 +616,10 @@ __device__ __forceinline__ Part join(const Part* parts, int n) {
   return r;
 }
 
-// Any row, logit by logit, by one CTA: rows with a NaN or +inf (results NaN, order over all values) and rows
-// that have nothing above kLow.  Slow, as such rows are rare: 151,936 fp16 logits at the lowest value 42 us, with
-// 20 alternatives 100 us (their largest in one pass of keys; a pass per alternative took 619 us), beside the 6 us
-// and 12 us of another row (device times in a graph).
+// Any row, logit by logit from memory, by one CTA: rows with a NaN or +inf (results NaN, order over all values),
+// rows whose maximum lies outside [kLowRow, kHighRow], and rows that lost a tile.  Slow, as such rows are rare:
+// 151,936 fp16 logits at the lowest value 42 us, with 20 alternatives 100 us (their largest in one pass of keys; a
+// pass per alternative took 619 us), beside the 6 us and 12 us of another row (device times in a graph).
 template <typename T>
 __device__ __noinline__ void general_row(Shared& sh, const Params& p, const void* x, int row, int head, int tok) {
   const int tid = threadIdx.x;
@@ -915,7 +915,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const _
     w += b.x + b.y;
     acc_s = acc_w = 0;
   };
-  bool lost = false;  // a tile never came: the row is wrong, and the warp asks for no more
+  bool lost = false;  // a tile never came: the warp asks for no more, and the row is taken from memory in the end
   for (int from = 0; from == 0 || (from < mine && !lost); from += kTileWords) {
     const int nw = mine - from;  // words from this tile on
     if (nw > 0 && !wait_full(&sh.full[warp], (from / kTileWords) & 1))
@@ -1044,7 +1044,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const _
     if (due) raise_threshold(sh, k);
   }
   flush();
-  if (lost && lane == 0 && p.error_bits) atomicOr(p.error_bits, kErrTimeout);
+  if (lost) {
+    s = __int_as_float(0x7fffffff);  // as a NaN among the logits does, it sends the row to general_row
+    if (lane == 0 && p.error_bits) atomicOr(p.error_bits, kErrTimeout);
+  }
   finish<T>(sh, p, m, mc, s, w, p_ref, given, above, ref_tile);
 }
 

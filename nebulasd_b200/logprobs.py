@@ -87,5 +87,6 @@ def _launch(logits, token_ids, num_top, rows, vocab, index) -> TokenLogprobs:
 
 def workspace_errors(device: torch.device | None = None) -> int:
     """Synchronise the device's current stream and return (and clear) the error bits that
-    calls on it recorded (bit 6: a token outside ``[-1, vocab)``; bit 3: a bounded wait gave up)."""
+    calls on it recorded (bit 6: a token outside ``[-1, vocab)``; bit 3: a bounded
+    wait gave up, and its row was read again, slowly)."""
     return _errors.read(device)
