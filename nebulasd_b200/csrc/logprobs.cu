@@ -392,7 +392,7 @@ __device__ __forceinline__ bool list_candidates(Shared& sh, int from, int words,
   const int first = sh.first_index[warp] + from * kPer;
   const int every = k <= 8 ? 8 : k <= 16 ? 16 : 32;
   const u64 thr = *static_cast<volatile u64*>(&sh.threshold);
-  if (*static_cast<volatile int*>(&sh.n) > kList) return false;
+  if (__any_sync(~0u, *static_cast<volatile int*>(&sh.n) > kList)) return false;  // (one answer for the warp)
   bool due = false;
   auto offer = [&](float f, int idx) {
     const u64 key = make_key(f, idx);
@@ -427,8 +427,10 @@ __device__ __forceinline__ bool list_candidates(Shared& sh, int from, int words,
 // threshold lower.
 __device__ __noinline__ void raise_threshold(Shared& sh, int num_top) {
   const int lane = threadIdx.x & 31;
-  const int n = min(*static_cast<volatile int*>(&sh.n), kList), from = max(0, n - kWindow);
-  unsigned int v[kWindow / 32], hi = 0, lo = reinterpret_cast<volatile unsigned int*>(&sh.threshold)[1], best = 0;
+  // (What others may change is read by one lane: the votes below need one course for the warp.)
+  const int n = min(__shfl_sync(~0u, *static_cast<volatile int*>(&sh.n), 0), kList), from = max(0, n - kWindow);
+  unsigned int lo = __shfl_sync(~0u, reinterpret_cast<volatile unsigned int*>(&sh.threshold)[1], 0);
+  unsigned int v[kWindow / 32], hi = 0, best = 0;
 #pragma unroll
   for (int i = 0; i < kWindow / 32; ++i) {
     const int at = from + lane + 32 * i;

@@ -105,6 +105,17 @@ def test_ties_and_order(dtype, cuda):
         _check(logits.to(dtype).to(cuda), tokens, k)
 
 
+@pytest.mark.parametrize("rows", [3, 500])
+@pytest.mark.parametrize("num_top", [1, 8, 9, 32])
+def test_lists_that_run_over(rows, num_top, cuda):
+    """Rising logits in every warp's range: candidates without end while other warps list and raise the threshold."""
+    vocab = 40009
+    at = torch.arange(vocab)
+    x = torch.stack([(at * (1 + r % 3) + 17 * r) % 4096 / 256.0 if r % 2 else at / vocab for r in range(rows)])
+    tokens = torch.arange(rows, dtype=torch.int32) * 79 % vocab
+    _check(x.float().to(cuda), tokens.to(cuda), num_top)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_masks(dtype, cuda):
     vocab, inf = 20011, math.inf
