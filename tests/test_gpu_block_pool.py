@@ -191,6 +191,30 @@ def test_fork_many(n, num_blocks, cuda):
     _fork(h, pool, [groups[i][0] for i in pick], empty, at, caps, cuda)
 
 
+def test_fork_many_that_meet(cuda):
+    """More children than the plan takes at a time: rows listed again, parents that are children and the reverse, on
+    both sides of the first 1,024; the free blocks run out among the later ones."""
+    n = 2300
+    pool, groups, empty = make_pool(17, num_blocks=3621, rows=2320, width=12, lens=[70, 100, 33, 160], layers=1, heads=1,
+                                    dim=8)
+    rng = np.random.default_rng(17)
+    parents = [groups[i][0] for i in rng.integers(0, 4, size=n)]
+    children, lens = empty[:n], [int(x) for x in rng.integers(1, 34, size=n)]
+    caps = [x + int(y) for x, y in zip(lens, rng.integers(0, 32, size=n))]
+    for i, j in ((1030, 3), (1500, 1023), (1024, 1023), (2100, 1500), (700, 20), (2290, 5)):
+        children[i] = children[j]                       # listed again
+    for i, j in ((1100, 8), (1800, 1700), (900, 30)):
+        parents[i] = children[j]                        # a child of this call
+    for i, j in ((9, 1200), (1050, 2000), (40, 60)):
+        parents[i] = children[j]                        # one of a later entry
+    lens[2200], caps[2200], lens[2250], caps[2250] = 16, 16, 0, 0  # need nothing, and get it
+    h = to_device(pool, cuda)
+    _fork(h, pool, parents, children, lens, caps, cuda)
+    held = pool.held[children]
+    assert (held[:1800] > 0).mean() > 0.98 and not held[2150:2200].any() and held[2200] == 1
+    assert int((pool.refs == 0).sum()) < 6
+
+
 # ------------------------------------------------------------------------ free
 def _free(h, pool, rows, dev):
     h.free(ints(rows, dev))
