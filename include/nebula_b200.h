@@ -331,12 +331,15 @@ int neb_rotary_inplace(void* q, void* k, const void* cos, const void* sin, int32
  * in use without a positive count, bit 8 too few free blocks, bit 9 copies in
  * conflict.  Calls on one pool must be ordered; no list may be part of the pool's
  * tables, and the tables may not overlap.  Fork and compact take pools of up to
- * 2^23 blocks. */
+ * 2^23 blocks.  A sequence takes all its blocks when it is forked or made
+ * (capacities); there is no call that gives a row in use one more. */
 
 /* Block dst[i] gets the first num_tokens[i] tokens (null: all) of block src[i],
  * all tiles, both planes; the rest of dst[i] keeps its contents.  A pair whose
  * dst is another pair's dst, or whose src is another pair's dst, is left out
- * (bit 9), one with a block or token count out of range too (bits 0, 4). */
+ * (bit 9), one with a block or token count out of range too (bits 0, 4).  Made
+ * for lists of up to some thousand pairs: the time spent on finding conflicts
+ * grows with their square. */
 int neb_copy_blocks(void* k_cache, void* v_cache, int64_t num_blocks, int32_t tiles_per_block,
                     int32_t block_size, int32_t token_bytes, const int32_t* src, const int32_t* dst,
                     const int32_t* num_tokens, int32_t num_pairs, uint32_t* error_bits, void* stream);

@@ -57,6 +57,8 @@ def copy_blocks(k_cache: torch.Tensor, v_cache: torch.Tensor, src: torch.Tensor,
     once, so a pair whose ``dst`` is another pair's ``dst``, or whose ``src`` is
     another pair's ``dst``, is left out and reported by ``workspace_errors``
     (bit 9), as is one with a block (bit 0) or token count (bit 4) out of range.
+    Lists of more than some thousand pairs are better split: finding conflicts
+    takes time with the square of their number.
     Runs on the current stream of the caches' device; its first call on a device
     must come before any graph capture.
     """
@@ -105,8 +107,11 @@ class BlockPool:
     ``ref_counts`` int32 ``[num_blocks]``: how many rows use each block.  All
     contiguous, on the caches' device.  Methods run on the current stream of
     that device, and calls on one pool must be ordered.  What they refuse they
-    leave as it was; ``errors`` tells why.  The tensors stay where they were when
-    the pool was made: with one replaced or moved, every method raises.
+    leave as it was; ``errors`` tells why.  Lists must not be parts of the pool's
+    own tensors.  A row gets all its blocks from the fork that makes it
+    (``capacities``); none of the methods gives a row in use one more.  The tensors
+    stay where they were when the pool was made: with one replaced or moved, every
+    method raises.
     """
 
     def __init__(self, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -148,9 +153,10 @@ class BlockPool:
 
         The child shares the parent's full blocks and gets fresh ones (lowest free first, in the order of
         the list) for the rest, the tokens of the partial block copied, so that both may append.  Length 0
-        makes a new sequence; its parent is not read.  Refused, leaving the child's row empty: a child that
-        is not empty or is listed before, a length beyond the parent's blocks (bit 4), rows out of range (bit
-        1), more than ``max_blocks`` blocks (bit 2), too few free blocks (bit 8).  Int32 vectors.
+        makes a new sequence; its parent is not read.  Refused, leaving the child's row as it was: a child
+        that is not empty or is listed before, a length beyond the parent's blocks (bit 4), rows out of range
+        (bit 1), more than ``max_blocks`` blocks (bit 2), too few free blocks (bit 8).  A parent's block that
+        no count vouches for is shared but not copied from (bit 7).  Int32 vectors.
         """
         self._check_tensors()
         index, n = self._index, children.numel()

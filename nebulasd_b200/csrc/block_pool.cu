@@ -29,9 +29,10 @@ constexpr int kLoads = 8;                          // 16-byte loads per lane in 
 // Copies of whole blocks run two CTAs per SM: 64 KB of loads in flight per SM, then as many stores (more, and
 // reads and writes alternate in shorter runs: 512 blocks of 1.2 MB per plane in items of 64 KB 392 us, with four
 // CTAs 415 us, with one 519 us).  Items of 128 KB copy scattered pairs best (383 us, 6.3 TB/s; 64 KB 395, 32 KB
-// 420), items of 32 KB the ascending ones of a compaction (2.4 GB moved, 768 us; 64 KB 777, 128 KB 786).  Partial
-// blocks have half the loads in flight per warp: four CTAs, items of one tile per warp (64 partial blocks of 28
-// layers 24 us, 5.2 TB/s; with two CTAs 27 us, with two tiles per warp 25 us).
+// 420), items of 32 KB the ascending ones of a compaction (2.4 GB moved, 768 us; 64 KB 777, 128 KB 786).  Items are
+// counted in tiles; these sizes are those of 4 KB tiles (16 tokens of 128 fp16).  Partial blocks have half the loads
+// in flight per warp: four CTAs, items of one tile per warp (64 partial blocks of 28 layers 24 us, 5.2 TB/s; with two
+// CTAs 27 us, with two tiles per warp 25 us).
 constexpr int kWholeCtas = 2, kWholeTiles = 4 * kCopyWarps, kMoveTiles = kCopyWarps;
 constexpr int kPartCtas = 4, kPartTiles = kCopyWarps;
 
@@ -94,7 +95,8 @@ struct Pair {
 // Copies all pairs' tiles, K plane before V plane, in items of kTiles tiles of one block and plane that go round
 // the CTAs, a tile per warp: what the GPU reads and writes at a time stays a few tens of MB of neighbouring
 // tiles.  (A range of tiles per warp instead: 2 to 6 % slower.)  load(i) fetches a pair, for the next item before
-// this one is copied (3 % of a compaction); keep(i, pair), called by the whole CTA, says whether it is copied.
+// this one is copied (3 % of a compaction; a fork's pair beyond its first 256 is two loads that depend on each
+// other, and they are waited for); keep(i, pair), called by the whole CTA, says whether it is copied.
 template <int kTiles, typename Load, typename Keep>
 __device__ __forceinline__ void copy_pairs(const Caches& c, int pairs, Load load, Keep keep) {
   const int words = c.token_bytes / 16, pitch = c.block_size * words, chunks = (c.tiles + kTiles - 1) / kTiles;
@@ -127,6 +129,9 @@ struct CopyParams {
   unsigned int* error_bits;
 };
 
+// Every item compares its pair with all destinations: one comparison per thread up to 256 pairs, and from there on
+// reads of the list that grow with the square of the pairs.  Of 36-layer blocks 4,096 pairs copy at 6.5 TB/s and
+// 16,384 at 5.9; of one-layer ones 4,096 at 4.8, 16,384 at 3.3 and 32,768 at 1.9.
 template <int kCtas, int kTiles>
 __global__ void __launch_bounds__(kCopyThreads, kCtas) copy_kernel(const __grid_constant__ CopyParams p) {
   const int own = (int)threadIdx.x < p.n ? p.dst[threadIdx.x] : -1;  // the thread's share of the first destinations

@@ -24,11 +24,14 @@
 // costs one comparison, now and then a candidate, and no barrier: 2,048 rows of
 // 151,936 fp16 logits list about 22 each for 5 alternatives, 90 for 20.
 //
-// What bounds it: HBM for many rows (2,048 of them: 110 us without alternatives,
-// 5.7 TB/s, 125 us with 5, 152 us with 20; reading them alone in this way takes
-// 105 us), with the XU pipe's exp2 (one per logit, 69 us) and about 8 instructions
-// per logit behind it.  For few rows, latency: one row 6.5 us, with 20 alternatives
-// 11.5 us, of which the launch, the first tile and the joins are all but 2 us.
+// What bounds it (device times in a graph): for many rows no unit alone.  2,048 of
+// them take 110 us without alternatives, 5.7 TB/s, 128 us with 5, 153 us with 20
+// (reading them alone in this way 105 us; exp2, one per logit, is 69 us of the XU
+// pipe); two full waves under the profiler keep HBM busy for 51 % of the time, the
+// issue slots for 57 % and XU for 54 %.  The rest is latency at the start and the
+// end of each row, which the other two CTAs of the SM hide in part.  For few rows
+// it is latency alone: one row 6.8 us, with 20 alternatives 12 us, of which the
+// launch, the first tile and the joins are all but 2 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -498,7 +501,9 @@ __device__ __noinline__ int collect(Shared& sh, const uint4* data, int words, in
 
 // Fills `sorted` from n to k with the logits below kLow, which the candidates leave out: largest first (all of
 // them mostly equal, -inf or another mask), then by index.  A pass over the row for the next lower value, four
-// words per thread in flight, and its first logits.
+// words per thread in flight, and its first logits: 5 allowed tokens of 151,936 with 20 alternatives take 19 us in
+// place of 13 (one row, the others -inf).  It is made for few distinct masked values: where each differs (x - 1e5
+// in fp32) there is a pass for every alternative that the allowed tokens do not fill, 3 ms for such a row.
 template <typename T>
 __device__ __noinline__ void fill_masked(Shared& sh, u64* sorted, const void* x, int vocab, int head, int n, int k) {
   constexpr int kPer = Elem<T>::kPerWord;
@@ -1053,8 +1058,12 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const _
   finish<T>(sh, p, m, mc, s, w, p_ref, given, above, ref_tile);
 }
 
-// CTAs per row: as many as the GPU holds at once for all rows (more, and a second round of them starts: 80 rows of
-// 151,936 fp16 logits 12.5 us with 320 CTAs, 15.6 us with 640), as long as each has kCtaBytes to read.
+// CTAs per row: as many as the GPU's places allow for all rows at once, as long as each has kCtaBytes to read.
+// Clusters leave places of a GPC empty that none of them fits into, so that the last few rows before a step run
+// after the others (151,936 fp16 logits, no alternatives: 48 rows of 8 CTAs 10.5 us, 53 to 55 of 8 14 us, 56 of 7
+// 11.4 us; 80 of 5 12.4 us, 88 of 5 15.2 us, 89 of 4 13.8 us).  From 223 rows on a row is one CTA's: up to 444
+// rows, the GPU's places, take about the same time (230 rows 22 us, 444 rows 29 us), and the next row starts a
+// second round (445 rows 38 us, 888 rows 52 us).
 constexpr int kCtaBytes = 16 * 1024;
 static int choose_splits(long long rows, int vocab, int item, int sms) {
   const long long by_size = ((long long)vocab * item + kCtaBytes - 1) / kCtaBytes;
